@@ -75,6 +75,11 @@ EXPORTS = (
     "lthc_interface_workspace_bytes",
     "lthc_interface_fwd",
     "lthc_interface_bwd",
+    "lthc_axial_rope",
+    "lthc_adamw_step",
+    "lthc_adamw_state_values",
+    "lthc_grad_norm_workspace_bytes",
+    "lthc_grad_norm",
 )
 
 _lib = None
@@ -95,8 +100,8 @@ def load() -> ctypes.CDLL:
             "(python -m flowmatching_lthc_amd._build); there is no CPU fallback"
         )
     lib = ctypes.CDLL(LIB_PATH)
-    vp, ci, i64, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
-    pp = ctypes.POINTER(ctypes.c_void_p)
+    vp, ci, i64, sz, f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_double
+    pp, pi = ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int64)
     lib.lthc_last_error.restype = ctypes.c_char_p
     lib.lthc_last_error.argtypes = []
     lib.lthc_abi_version.restype = ci
@@ -157,6 +162,14 @@ def load() -> ctypes.CDLL:
         "lthc_block_tail_fwd": [
             vp, vp, vp, vp, ci, vp, ci, vp, ci, vp, vp, i64, vp, vp, vp, i64, i64, i64, ctypes.c_float, vp,
         ],  # fmt: skip
+        "lthc_axial_rope": [
+            vp, vp, pi, i64, vp, vp, pi, i64, ci, vp, ci, pi, vp, pi, i64, ci, ci, i64, i64, i64, vp,
+        ],  # fmt: skip
+        "lthc_adamw_step": [
+            pp, ci, pp, ci, pp, pp, ci, pp, pp, pp, pi, i64, f64, f64, f64, f64, f64, f64, f64, vp, vp, vp, f64, vp,
+        ],  # fmt: skip
+        "lthc_adamw_state_values": [pp, pp, pp, pp, pp, pi, i64, vp],
+        "lthc_grad_norm": [pp, ci, pi, i64, vp, vp, sz, vp],
         "lthc_norm_modulate_bwd": [vp, vp, ci, vp, ci, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp],
     }
     for name, args in sig.items():
@@ -189,6 +202,8 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name + "_workspace_bytes")
         fn.argtypes = [i64, i64, i64]
         fn.restype = sz
+    lib.lthc_grad_norm_workspace_bytes.argtypes = [pi, i64]
+    lib.lthc_grad_norm_workspace_bytes.restype = sz
     _lib = lib
     return lib
 

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <optional>
@@ -960,6 +961,253 @@ std::tuple<Tensor, Tensor, Tensor> block_tail_cuda(const Tensor& z_, const Tenso
 }
 
 // ---------------------------------------------------------------------------
+// rotary positions with several axes
+// ---------------------------------------------------------------------------
+int position_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kInt: return LTHC_POS_I32;
+    case at::kLong: return LTHC_POS_I64;
+    case at::kFloat: return LTHC_POS_F32;
+    case at::kDouble: return LTHC_POS_F64;
+    default: break;
+  }
+  TORCH_CHECK_VALUE(false, "positions must be int32, int64, float32 or float64, got ", t.scalar_type());
+}
+
+int64_t check_rope(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
+                   bool interleaved) {
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+                    "q and k must be [B,N,H,D] with heads of their own, got ", shape(q), " and ", shape(k));
+  TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type(), "q and k must have one dtype, got ", q.scalar_type(), ", ", k.scalar_type());
+  code(q);
+  const int64_t axes = static_cast<int64_t>(sections.size());
+  int64_t rotated = 0;
+  for (const int64_t s : sections) {
+    TORCH_CHECK_VALUE(s > 0 && s % 2 == 0, "sections must be positive and even, got ", sections);
+    rotated += s;
+  }
+  TORCH_CHECK_VALUE(axes >= 1 && axes <= 4 && rotated <= q.size(3) && rotated <= 1024, "1 to 4 sections of at most the head's ",
+                    q.size(3), " channels (and 1024) expected, got ", sections);
+  TORCH_CHECK_VALUE(!interleaved || q.size(3) % 2 == 0, "interleaved pairs need an even head width, got ", q.size(3));
+  TORCH_CHECK_VALUE(has_shape(inv_freq, {rotated / 2}) && inv_freq.scalar_type() == at::kDouble, "inv_freq must be float64 [",
+                    rotated / 2, "], got ", shape(inv_freq), " ", inv_freq.scalar_type());
+  position_code(positions);
+  TORCH_CHECK_VALUE(has_shape(positions, {q.size(1), axes}) || has_shape(positions, {q.size(0), q.size(1), axes}),
+                    "positions must be [", q.size(1), ",", axes, "] or [", q.size(0), ",", q.size(1), ",", axes, "], got ",
+                    shape(positions));
+  return axes;
+}
+
+// A head's channels consecutive, and for interleaved pairs every address even.
+Tensor rope_operand(const Tensor& t, bool interleaved) {
+  bool ok = t.stride(3) == 1 || t.size(3) == 1;
+  if (interleaved) {
+    ok = ok && aligned(t, 2 * t.element_size());
+    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 2 == 0;
+  }
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void launch_rope(const Tensor& q, const Tensor& qo, const Tensor& k, const Tensor& ko, const Tensor& positions,
+                 const Tensor& inv_freq_, at::IntArrayRef sections, bool interleaved, bool inverse) {
+  auto strides = [](const Tensor& x, const Tensor& y) {
+    return std::array<int64_t, 6>{x.stride(0), x.stride(1), x.stride(2), y.stride(0), y.stride(1), y.stride(2)};
+  };
+  const auto qs = strides(q, qo), ks = strides(k, ko);
+  const bool each = positions.dim() == 3;
+  const std::array<int64_t, 3> ps{each ? positions.stride(0) : 0, positions.stride(-2), positions.stride(-1)};
+  const Tensor inv_freq = inv_freq_.contiguous();
+  const Launch l(q);
+  check(lthc_axial_rope(data(q), data(qo), qs.data(), q.size(2), data(k), data(ko), ks.data(), k.size(2), code(q),
+                        data(positions), position_code(positions), ps.data(), static_cast<const double*>(data(inv_freq)),
+                        sections.data(), static_cast<int64_t>(sections.size()), interleaved, inverse, q.size(0), q.size(1),
+                        q.size(3), l.stream),
+        "lthc_axial_rope");
+}
+
+std::tuple<Tensor, Tensor> axial_rope_cuda(const Tensor& q_, const Tensor& k_, const Tensor& positions, const Tensor& inv_freq,
+                                           at::IntArrayRef sections, bool interleaved, bool inverse) {
+  on_gpu(q_, k_, positions, inv_freq);
+  check_rope(q_, k_, positions, inv_freq, sections, interleaved);
+  Tensor qo = at::empty_like(q_), ko = at::empty_like(k_);
+  // an output in its input's layout whose channels are not consecutive goes through a contiguous one
+  const Tensor q = rope_operand(q_, interleaved), k = rope_operand(k_, interleaved);
+  Tensor qt = rope_operand(qo, interleaved), kt = rope_operand(ko, interleaved);
+  launch_rope(q, qt, k, kt, positions, inv_freq, sections, interleaved, inverse);
+  if (!qt.is_same(qo)) qo.copy_(qt);
+  if (!kt.is_same(ko)) ko.copy_(kt);
+  return {qo, ko};
+}
+
+// ---------------------------------------------------------------------------
+// AdamW over many tensors
+// ---------------------------------------------------------------------------
+constexpr int64_t kAdamRun = 256;  // elements that share a scale of an 8-bit state
+
+// One device, one of the dtypes for all.
+void check_many(TensorList ts, const char* name, const Tensor& first, size_t count, std::initializer_list<at::ScalarType> dtypes) {
+  TORCH_CHECK_VALUE(ts.size() == count, "expected ", count, " ", name, ", got ", ts.size());
+  for (const Tensor& t : ts) {
+    on_gpu(first, t);
+    TORCH_CHECK_VALUE(t.scalar_type() == ts[0].scalar_type(), name, " must have one dtype, got ", ts[0].scalar_type(), ", ",
+                      t.scalar_type());
+  }
+  TORCH_CHECK_VALUE(std::find(dtypes.begin(), dtypes.end(), ts[0].scalar_type()) != dtypes.end(), "unsupported dtype of ", name,
+                    ": ", ts[0].scalar_type());
+}
+
+void same_layout(TensorList ts, TensorList params, const char* name) {
+  for (size_t i = 0; i < ts.size(); ++i)
+    TORCH_CHECK_VALUE(ts[i].sizes() == params[i].sizes() && (ts[i].strides() == params[i].strides() ||
+                                                             (ts[i].is_contiguous() && params[i].is_contiguous())),
+                      name, " ", i, " must have its parameter's sizes ", params[i].sizes(), " and strides ", params[i].strides(),
+                      ", got ", ts[i].sizes(), ", ", ts[i].strides());
+}
+
+// Every tensor that the step writes has its memory for itself (the kernels' blocks run in no order).
+void no_overlap(std::initializer_list<TensorList> lists) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (const TensorList l : lists)
+    for (const Tensor& t : l)
+      if (t.numel() > 0) {
+        const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+        spans.emplace_back(at, at + t.numel() * t.element_size());
+      }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "tensors that the step writes overlap (the same tensor twice?)");
+}
+
+void written(TensorList ts) {
+  for (const Tensor& t : ts)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+const float* device_scalar(const std::optional<Tensor>& t, const Tensor& like, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  on_gpu(like, *t);
+  TORCH_CHECK_VALUE(t->numel() == 1 && t->scalar_type() == at::kFloat, name, " must be one float32, got ", shape(*t), " ",
+                    t->scalar_type());
+  return static_cast<const float*>(data(*t));
+}
+
+std::vector<int64_t> numels(TensorList ts) {
+  std::vector<int64_t> n;
+  for (const Tensor& t : ts) n.push_back(t.numel());
+  return n;
+}
+
+void check_8bit(TensorList params, TensorList avgs, TensorList sqs, TensorList scales, const Tensor& first) {
+  check_many(avgs, "exp_avgs", first, params.size(), {at::kChar});
+  check_many(sqs, "exp_avg_sqs", first, params.size(), {at::kByte});
+  check_many(scales, "scales", first, params.size(), {at::kFloat});
+  for (size_t i = 0; i < params.size(); ++i) {
+    const int64_t n = params[i].numel(), runs = (n + kAdamRun - 1) / kAdamRun;
+    TORCH_CHECK_VALUE(avgs[i].numel() == n && sqs[i].numel() == n && avgs[i].is_contiguous() && sqs[i].is_contiguous(),
+                      "8-bit states of tensor ", i, " must be contiguous with ", n, " codes");
+    TORCH_CHECK_VALUE(has_shape(scales[i], {2, runs}) && scales[i].is_contiguous(), "scales of tensor ", i, " must be [2,", runs,
+                      "], got ", shape(scales[i]));
+  }
+}
+
+void adamw_step_cuda(TensorList params, TensorList grads_, TensorList avgs, TensorList sqs, TensorList scales, TensorList masters,
+                     TensorList emas, double step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                     double ema_decay, const std::optional<Tensor>& device_step, const std::optional<Tensor>& device_lr,
+                     const std::optional<Tensor>& grad_norm, double max_norm) {
+  if (params.empty()) return;
+  const Tensor& first = params[0];
+  const auto any = {at::kFloat, at::kBFloat16, at::kHalf};
+  check_many(params, "params", first, params.size(), any);
+  check_many(grads_, "grads", first, params.size(), any);
+  const bool bits8 = !scales.empty();
+  if (bits8) {
+    check_8bit(params, avgs, sqs, scales, first);
+  } else {
+    check_many(avgs, "exp_avgs", first, params.size(), {at::kFloat});
+    check_many(sqs, "exp_avg_sqs", first, params.size(), {at::kFloat});
+    same_layout(avgs, params, "exp_avg");
+    same_layout(sqs, params, "exp_avg_sq");
+  }
+  if (!masters.empty()) {
+    check_many(masters, "masters", first, params.size(), {at::kFloat});
+    same_layout(masters, params, "master");
+  }
+  if (!emas.empty()) {
+    check_many(emas, "emas", first, params.size(), {at::kFloat});
+    same_layout(emas, params, "ema");
+  }
+  std::vector<Tensor> grads;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor &p = params[i], &g = grads_[i];
+    TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "parameter ", i, " must fill its memory (strides ", p.strides(), ")");
+    TORCH_CHECK_VALUE(g.sizes() == p.sizes(), "gradient ", i, " must be ", p.sizes(), ", got ", g.sizes());
+    const bool as_is = g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous());
+    grads.push_back(as_is ? g : at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g));
+  }
+  no_overlap({params, avgs, sqs, scales, masters, emas});
+  const float* dstep = device_scalar(device_step, first, "step");
+  const float* dlr = device_scalar(device_lr, first, "lr");
+  const float* norm = device_scalar(grad_norm, first, "grad_norm");
+  const auto n = numels(params);
+  const auto p = pointers<void>(params), m = pointers<void>(avgs), v = pointers<void>(sqs);
+  const auto g = pointers(grads);
+  auto floats = [](TensorList ts) {
+    std::vector<float*> out;
+    for (const Tensor& t : ts) out.push_back(static_cast<float*>(t.data_ptr()));
+    return out;
+  };
+  const auto sc = floats(scales), ma = floats(masters), em = floats(emas);
+  const Launch l(first);
+  check(lthc_adamw_step(p.data(), code(first), g.data(), code(grads[0]), m.data(), v.data(), bits8 ? 8 : 32,
+                        bits8 ? sc.data() : nullptr, masters.empty() ? nullptr : ma.data(), emas.empty() ? nullptr : em.data(),
+                        n.data(), static_cast<int64_t>(n.size()), step, lr, beta1, beta2, eps, weight_decay, ema_decay, dstep,
+                        dlr, norm, max_norm, l.stream),
+        "lthc_adamw_step");
+  for (const TensorList t : {params, avgs, sqs, scales, masters, emas}) written(t);
+}
+
+std::tuple<std::vector<Tensor>, std::vector<Tensor>> adamw_state_values_cuda(TensorList avgs, TensorList sqs, TensorList scales) {
+  std::vector<Tensor> m, v;
+  if (avgs.empty()) return {m, v};
+  const Tensor& first = avgs[0];
+  check_8bit(avgs, avgs, sqs, scales, first);
+  for (const Tensor& t : avgs) {
+    m.push_back(fp32_like(t.sizes(), t));
+    v.push_back(fp32_like(t.sizes(), t));
+  }
+  const auto n = numels(avgs);
+  const auto a = pointers(avgs), b = pointers(sqs);
+  std::vector<const float*> s;
+  std::vector<float*> om, ov;
+  for (size_t i = 0; i < n.size(); ++i) {
+    s.push_back(static_cast<const float*>(data(scales[i])));
+    om.push_back(static_cast<float*>(data(m[i])));
+    ov.push_back(static_cast<float*>(data(v[i])));
+  }
+  const Launch l(first);
+  check(lthc_adamw_state_values(a.data(), b.data(), s.data(), om.data(), ov.data(), n.data(), static_cast<int64_t>(n.size()),
+                                l.stream),
+        "lthc_adamw_state_values");
+  return {m, v};
+}
+
+Tensor grad_norm_cuda(TensorList grads_) {
+  TORCH_CHECK_VALUE(!grads_.empty(), "grad_norm of no tensors");
+  check_many(grads_, "grads", grads_[0], grads_.size(), {at::kFloat, at::kBFloat16, at::kHalf});
+  std::vector<Tensor> grads;
+  for (const Tensor& g : grads_) grads.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
+  const auto n = numels(grads);
+  const auto g = pointers(grads);
+  Tensor out = fp32_like({}, grads[0]);
+  const Tensor ws = workspace(lthc_grad_norm_workspace_bytes(n.data(), static_cast<int64_t>(n.size())), out);
+  const Launch l(out);
+  check(lthc_grad_norm(g.data(), code(grads[0]), n.data(), static_cast<int64_t>(n.size()), static_cast<float*>(data(out)),
+                       data(ws), ws.numel(), l.stream),
+        "lthc_grad_norm");
+  return out;
+}
+
+// ---------------------------------------------------------------------------
 // autograd
 // ---------------------------------------------------------------------------
 // The dispatcher's handle of an operator, looked up once.
@@ -1030,6 +1278,8 @@ LTHC_REPLAY(replay_qk, "qk_norm_rope")
 LTHC_REPLAY(replay_attention, "qk_norm_rope_attention")
 LTHC_REPLAY(replay_swiglu, "swiglu")
 LTHC_REPLAY(replay_ganm, "gate_add_norm_modulate")
+LTHC_OP(op_axial_rope, "axial_rope",
+        std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, at::IntArrayRef, bool, bool))
 LTHC_OP(op_linear_weight_grad, "linear_weight_grad", std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, bool))
 
 using BelowAutograd = at::AutoDispatchBelowADInplaceOrView;
@@ -1578,6 +1828,31 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
+// The gradient of a rotation is the rotation by the negative angle.  A side whose gradient is not asked for takes part
+// with no heads.
+struct AxialRopeFn : torch::autograd::Function<AxialRopeFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions,
+                               const Tensor& inv_freq, at::IntArrayRef sections, bool interleaved, bool inverse) {
+    BelowAutograd below;
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["sections"] = sections.vec();
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    auto [qo, ko] = op_axial_rope().call(q, k, positions, inv_freq, sections, interleaved, inverse);
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    BackwardScope scope;
+    const auto s = ctx->get_saved_variables();
+    const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1);
+    auto part = [](const Tensor& g, bool need) { return need ? g : g.narrow(2, 0, 0); };
+    auto [gq, gk] = op_axial_rope().call(part(grads[0], need_q), part(grads[1], need_k), s[0], s[1],
+                                         ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(),
+                                         !ctx->saved_data["inverse"].toBool());
+    return {need_q ? gq : Tensor(), need_k ? gk : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---- autograd kernels: record a node, or go straight below autograd
 Tensor read_autograd(const Tensor& x, const Tensor& w) {
   if (recording(x, w)) return ReadFn::apply(x, w);
@@ -1693,6 +1968,14 @@ Tensor gres_autograd(const Tensor& d, const Tensor& gate, const Tensor& m) {
   return op_gres().call(d, gate, m);
 }
 
+std::tuple<Tensor, Tensor> axial_rope_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                               at::IntArrayRef sections, bool interleaved, bool inverse) {
+  TORCH_CHECK_VALUE(!recording(positions, inv_freq), "axial_rope gives no gradient of positions or inv_freq");
+  if (recording(q, k)) return pair(AxialRopeFn::apply(q, k, positions, inv_freq, sections, interleaved, inverse));
+  BelowAutograd below;
+  return op_axial_rope().call(q, k, positions, inv_freq, sections, interleaved, inverse);
+}
+
 // Composite ops: they only open an autograd node around registered ops.
 std::tuple<Tensor, Tensor> read_with_residual(const Tensor& x, const Tensor& weight) {
   return pair(OpenFn::apply(x, weight));
@@ -1769,6 +2052,10 @@ TORCH_LIBRARY_IMPL(jit_thc, CUDA, m) {
   m.impl("gate_residual_backward", gate_residual_backward_cuda);
   m.impl("linear_weight_grad", linear_weight_grad_cuda);
   m.impl("block_tail", block_tail_cuda);
+  m.impl("axial_rope", axial_rope_cuda);
+  m.impl("adamw_step", adamw_step_cuda);
+  m.impl("adamw_state_values", adamw_state_values_cuda);
+  m.impl("grad_norm", grad_norm_cuda);
 }
 
 // The nodes hold no device code: meta tensors, fake ones of any device and CPU tensors (whose kernels refuse them, or are
@@ -1791,6 +2078,7 @@ static void autograd_kernels(torch::Library& m) {
   m.impl("swiglu", swiglu_autograd);
   m.impl("gate_add_norm_modulate", ganm_autograd);
   m.impl("gate_residual", gres_autograd);
+  m.impl("axial_rope", axial_rope_autograd);
 }
 
 TORCH_LIBRARY_IMPL(jit_thc, AutogradCUDA, m) { autograd_kernels(m); }

@@ -24,7 +24,12 @@ activation dtype), registered as a ``jit_thc`` custom op:
   and the next block's first pre-norm (:315-317) in one pass, each value
   that of the three separate ops.
 
-Every op but block_tail (inference only) has a backward kernel of its own,
+Two more have no eager sequence in the reference's branch:
+
+* ``jit_thc::axial_rope``: rotary positions with several axes on q and k, for token maps that
+  VisionRotaryEmbeddingFast's square grid does not describe (frames, oblong maps, single tokens).
+
+Every op above but block_tail (inference only) has a backward kernel of its own,
 ``jit_thc::<op>_backward``, one HIP pass that recomputes what it needs from the
 op's inputs and gives the gradients of the eager sequence.  For batched
 gradients (is_grads_batched, vmap) torch runs that pass once per sample.  A
@@ -34,6 +39,8 @@ compiled graph keeps the chain's intermediates in fp32.
 """
 
 from __future__ import annotations
+
+from collections.abc import Sequence
 
 import torch
 import torch.nn.functional as F
@@ -363,6 +370,31 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor | None:
     if dt not in (torch.bfloat16, torch.float16) or weight.device != x.device:
         return None
     return torch.ops.jit_thc.linear(x, weight, bias)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions with several axes
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("jit_thc::axial_rope", mutates_args=())
+def axial_rope(
+    q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[int], interleaved: bool = True,
+    inverse: bool = False,
+) -> tuple[Tensor, Tensor]:
+    """(q, k) [B, N, Hq | Hk, D] turned by their tokens' positions on several axes (time, height, width), in q's dtype, one
+    pass over both.
+
+    The first R = sum(sections) channels of a head are R / 2 pairs: interleaved (2p, 2p + 1), as VisionRotaryEmbeddingFast
+    pairs them, else (p, p + R / 2).  Pair p belongs to the axis whose section it lies in (sections[a] channels, even, 1 to 4
+    axes) and turns by the angle positions[..., a] * inv_freq[p], a product in 64 bits; the channels past R are copied.
+    positions [N, A] (one map for the batch) or [B, N, A], int32, int64, float32 or float64; inv_freq float64 [R / 2].
+    inverse: by the negative angle, which is the gradient's rotation.  Heads with 0 entries are left out.  Outputs have
+    their inputs' layout where that is dense, and are contiguous otherwise.  No gradient of positions or inv_freq."""
+    _refuse(q)
+
+
+@_fake(axial_rope)
+def _(q, k, positions, inv_freq, sections, interleaved=True, inverse=False):
+    return torch.empty_like(q), torch.empty_like(k)
 
 
 # ---------------------------------------------------------------------------

@@ -568,6 +568,66 @@ int lthc_interface_bwd(const void* gx, const void* const* gz, int x_dtype, const
                        float* dalpha, float* dbeta, int64_t B, int64_t G, int64_t s, int64_t C, int L, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/*
+ * ROTARY POSITIONS WITH SEVERAL AXES (no reference op: VisionRotaryEmbeddingFast,
+ * jit_shared_adaln.py:33-59, has two axes and a table of one square grid).  For
+ * q and k, B x N tokens of q_heads and k_heads heads of D channels (x_dtype):
+ * the first R = sum of `sections` channels of a head are R / 2 pairs, pair p of
+ * the axis whose section it lies in (sections: `axes` <= 4 even host values, R
+ * <= D, R <= 1024), turned by the angle positions[b, n, axis(p)] * inv_freq[p]:
+ *   y0 = x0 cos - x1 sin, y1 = x0 sin + x1 cos
+ * with (x0, x1) = channels (2p, 2p + 1) where `interleaved`, else (p, p + R/2);
+ * the channels past R are copied.  `inverse` turns by the negative angle (the
+ * gradient).  inv_freq is double [R / 2]; angles are products in 64 bits.
+ * *_strides are six host values in elements: (batch, token, head) of the input,
+ * then of the output; the channels of a head are consecutive.  pos_strides: (batch, token,
+ * axis), 0 for a dimension that is shared.  An output may be its input.  A side with 0
+ * heads is left out.  interleaved: D and the strides even, addresses aligned to
+ * 2 elements.
+ */
+#define LTHC_POS_I32 0
+#define LTHC_POS_I64 1
+#define LTHC_POS_F32 2
+#define LTHC_POS_F64 3
+int lthc_axial_rope(const void* q, void* q_out, const int64_t* q_strides, int64_t q_heads, const void* k, void* k_out,
+                    const int64_t* k_strides, int64_t k_heads, int x_dtype, const void* positions, int pos_dtype,
+                    const int64_t* pos_strides, const double* inv_freq, const int64_t* sections, int64_t axes,
+                    int interleaved, int inverse, int64_t B, int64_t N, int64_t D, void* stream);
+
+/*
+ * ADAMW STEP OVER MANY TENSORS (no reference op: torch.optim.AdamW and the EMA
+ * of the reference's training script).  `count` tensors of numels[i] elements,
+ * given by host arrays of device pointers; in place, fp32 arithmetic:
+ *   g = clip g;  m = m beta1 + g (1 - beta1);  v = v beta2 + g^2 (1 - beta2)
+ *   p = p (1 - lr wd) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ *   ema = ema d + p (1 - d)
+ * params (p_dtype) and grads (g_dtype) have one dtype each.  masters (NULL:
+ * none; 16-bit parameters only): fp32 copies that take the step and are rounded
+ * into the parameters.  emas (NULL: none): fp32.  state_bits 32: exp_avgs and
+ * exp_avg_sqs are fp32.  8: they are int8 and uint8 codes of runs of 256
+ * elements (the last one may be shorter), scales[i] fp32 [2, runs] = (A, B):
+ *   m = A c |c| / 127^2,  v = B (c / 255)^4
+ * grad_norm (NULL: no clipping): the norm of all gradients on the device; clip =
+ * min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves every
+ * tensor as it is.  device_step and device_lr (fp32, NULL: `step` and `lr`) are
+ * read when the kernels run.  No tensor may overlap another.
+ */
+int lthc_adamw_step(void* const* params, int p_dtype, const void* const* grads, int g_dtype, void* const* exp_avgs,
+                    void* const* exp_avg_sqs, int state_bits, float* const* scales, float* const* masters,
+                    float* const* emas, const int64_t* numels, int64_t count, double step, double lr, double beta1,
+                    double beta2, double eps, double weight_decay, double ema_decay, const float* device_step,
+                    const float* device_lr, const float* grad_norm, double max_norm, void* stream);
+
+/* The fp32 values of 8-bit states (above). */
+int lthc_adamw_state_values(const void* const* exp_avgs, const void* const* exp_avg_sqs, const float* const* scales,
+                            float* const* out_avgs, float* const* out_sqs, const int64_t* numels, int64_t count,
+                            void* stream);
+
+/* out = sqrt(sum of squares over all `count` tensors), summed in 64 bits in a fixed order. */
+size_t lthc_grad_norm_workspace_bytes(const int64_t* numels, int64_t count);
+int lthc_grad_norm(const void* const* grads, int g_dtype, const int64_t* numels, int64_t count, float* out,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

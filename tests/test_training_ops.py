@@ -1,0 +1,245 @@
+"""Refusals, fakes and host logic of the training step's operators: CPU only, no kernel runs."""
+
+from __future__ import annotations
+
+import copy
+import ctypes
+
+import pytest
+import torch
+
+from flowmatching_lthc_amd import _abi, optim
+from flowmatching_lthc_amd import ops_branch as OB
+
+
+def err(rc):
+    return rc, _abi.load().lthc_last_error().decode()
+
+
+FAKE = ctypes.c_void_p(4096)  # never dereferenced: the checks fail first
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def rope(sections=(32, 32), D=64, heads=2, N=4, dtype=_abi.BF16, q=FAKE, interleaved=1, strides=None, pos=1, axes=None, B=2):
+    s = strides or i64(N * heads * D, heads * D, D, N * heads * D, heads * D, D)
+    n = len(sections) if axes is None else axes
+    return err(_abi.load().lthc_axial_rope(q, FAKE, s, heads, FAKE, FAKE, s, heads, dtype, FAKE, pos, i64(0, n, 1), FAKE,
+                                           i64(*sections), n, interleaved, 0, B, N, D, None))  # fmt: skip
+
+
+def test_axial_rope_refusals_of_the_c_entry():
+    for kw, text in (
+        (dict(sections=(31, 32)), "even"),
+        (dict(sections=(0, 32)), "even"),
+        (dict(sections=(64, 32)), "wider"),
+        (dict(sections=(2,) * 5), "axes"),
+        (dict(axes=0), "axes"),
+        (dict(dtype=5), "dtype"),
+        (dict(pos=9), "position"),
+        (dict(q=None), "NULL"),
+        (dict(q=ctypes.c_void_p(4097)), "misaligned"),
+        (dict(q=ctypes.c_void_p(4098)), "even"),
+        (dict(strides=i64(8, 65, 64, 8, 64, 64)), "even"),
+        (dict(D=65, strides=i64(520, 130, 65, 520, 130, 65)), "even"),
+        (dict(sections=(1024, 1024), D=2048), "wide"),
+        (dict(B=-1), "negative"),
+        (dict(N=1 << 31), "tokens"),
+    ):
+        rc, msg = rope(**kw)
+        assert rc in (_abi.ERR_INVALID, _abi.ERR_UNSUPPORTED) and text in msg, (kw, rc, msg)
+    assert rope(B=0)[0] == _abi.OK and rope(N=0)[0] == _abi.OK and rope(heads=0)[0] == _abi.OK
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(shape, device="meta", dtype=dtype)
+
+
+def test_axial_rope_refuses_cpu_tensors_and_predicts_its_outputs():
+    q = torch.zeros(1, 4, 2, 8)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        OB.axial_rope(q, q, torch.zeros(4, 1), torch.zeros(2, dtype=torch.float64), (4,))
+    x = meta(2, 3, 4, 10, 16, dtype=torch.bfloat16)
+    q, k = x.select(2, 0), meta(2, 10, 3, 16).transpose(1, 2)
+    a, b = torch.ops.jit_thc.axial_rope(q, k, meta(3, 2), meta(4, dtype=torch.float64), [4, 4], True, False)
+    assert a.shape == q.shape and a.is_contiguous() and b.stride() == k.stride()
+
+
+def test_axial_rope_has_no_gradient_of_positions():
+    q = torch.zeros(1, 4, 2, 8, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        OB.axial_rope(q, q, torch.zeros(4, 1, requires_grad=True), torch.zeros(2, dtype=torch.float64), (4,))
+
+
+# ---------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------
+def adamw(n=1, numel=8, p=4096, dtype=_abi.F32, g=_abi.F32, bits=32, scales=None, masters=None, step=1.0, b1=0.9, norm=None, max_norm=1.0, eps=1e-8, ema=0.5):
+    arr = (ctypes.c_void_p * n)(*([4096] * n))
+    ps = (ctypes.c_void_p * n)(*([p] * n))
+    return err(_abi.load().lthc_adamw_step(ps, dtype, arr, g, arr, arr, bits, scales, masters, None, i64(*([numel] * n)), n, step,
+                                           1e-3, b1, 0.99, eps, 0.0, ema, None, None, norm, max_norm, None))  # fmt: skip
+
+
+def test_adamw_refusals_of_the_c_entries():
+    arr = (ctypes.c_void_p * 1)(4096)
+    for kw, text in (
+        (dict(dtype=4), "dtype"),
+        (dict(bits=16), "32 or 8"),
+        (dict(bits=8), "scales"),
+        (dict(p=0), "NULL"),
+        (dict(p=4098), "misaligned"),
+        (dict(numel=-1), "numel"),
+        (dict(step=0.0), "step"),
+        (dict(b1=1.0), "betas"),
+        (dict(eps=-1.0), "eps"),
+        (dict(eps=float("nan")), "eps"),
+        (dict(ema=1.5), "ema"),
+        (dict(masters=arr), "16-bit"),
+        (dict(norm=4096, max_norm=0.0), "max_norm"),
+    ):
+        rc, msg = adamw(**kw)
+        assert rc in (_abi.ERR_INVALID, _abi.ERR_UNSUPPORTED) and text in msg, (kw, rc, msg)
+    assert adamw(n=0)[0] == _abi.OK
+    assert adamw(numel=0, p=0)[0] == _abi.OK  # empty tensors need no memory
+    lib = _abi.load()
+    need = lib.lthc_grad_norm_workspace_bytes(i64(5), 1)
+    assert need > 0
+    rc, msg = err(lib.lthc_grad_norm(arr, _abi.F32, i64(5), 1, 4096, 4096, need - 1, None))
+    assert rc == _abi.ERR_INVALID and "workspace" in msg
+    rc, msg = err(lib.lthc_grad_norm(arr, _abi.F32, i64(5), 1, None, 4096, need, None))
+    assert rc == _abi.ERR_INVALID and "out" in msg
+    # many tensors: a place of its own for every launch's partial sums
+    assert lib.lthc_grad_norm_workspace_bytes(i64(*([5] * 1001)), 1001) >= 6 * need
+    rc, msg = err(lib.lthc_adamw_state_values(arr, arr, arr, arr, (ctypes.c_void_p * 1)(2), i64(5), 1, None))
+    assert rc == _abi.ERR_INVALID and "misaligned" in msg
+
+
+def test_adamw_refuses_cpu_tensors_and_bad_options():
+    t = [torch.zeros(3)]
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        optim.adamw_step(t, t, t, t, step=1)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        optim.grad_norm(t)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        optim.state_values(t, t, t)
+    for kw in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(state_bits=4), dict(ema_decay=2.0),
+               dict(max_norm=0.0), dict(lr=torch.tensor(1e-3))):  # fmt: skip
+        with pytest.raises(ValueError):
+            optim.AdamW([torch.nn.Parameter(torch.zeros(2))], **kw)
+
+
+# ---- the class on stand-in kernels
+def plain_step(params, grads, avgs, sqs, scales, masters, emas, step, lr, b1, b2, eps, wd, d, dstep, dlr, norm, max_norm):
+    step, lr = (step if dstep is None else float(dstep)), (lr if dlr is None else float(dlr))
+    for i, (p, g, m, v) in enumerate(zip(params, grads, avgs, sqs)):
+        if scales:
+            raise NotImplementedError
+        g = g.float() * (1.0 if norm is None else min(1.0, max_norm / (float(norm) + 1e-6)))
+        m.mul_(b1).add_(g, alpha=1 - b1)
+        v.mul_(b2).add_(g * g, alpha=1 - b2)
+        w = masters[i] if masters else p.float()
+        w = w * (1 - lr * wd) - lr / (1 - b1**step) * m / ((v / (1 - b2**step)).sqrt() + eps)
+        if masters:
+            masters[i].copy_(w)
+        p.copy_(w)
+        if emas:
+            emas[i].mul_(d).add_(w, alpha=1 - d)
+
+
+@pytest.fixture
+def cpu_kernels():
+    lib = torch.library.Library("jit_thc", "IMPL")
+    lib.impl("adamw_step", plain_step, "CPU")
+    lib.impl("grad_norm", lambda gs: torch.linalg.vector_norm(torch.cat([g.float().flatten() for g in gs])), "CPU")
+    yield
+    lib._destroy()
+
+
+def parameters(seed, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=gen).to(dtype)) for s in ((4, 3), (7,), (2, 2, 2))]
+
+
+def run(opt, params, steps, seed=100, skip=()):
+    for t in range(steps):
+        gen = torch.Generator().manual_seed(seed + t)
+        for i, p in enumerate(params):
+            g = torch.randn(p.shape, generator=gen).to(p.dtype)
+            p.grad = None if (t, i) in skip else g
+        opt.step()
+
+
+def test_adamw_takes_torch_adamws_steps(cpu_kernels):
+    """Parameters without a gradient on some steps too: each counts its own steps."""
+    ours, theirs = parameters(0), parameters(0)
+    a = optim.AdamW(ours, lr=1e-2, betas=(0.8, 0.9), weight_decay=0.1)
+    b = torch.optim.AdamW(theirs, lr=1e-2, betas=(0.8, 0.9), weight_decay=0.1)
+    for opt, ps in ((a, ours), (b, theirs)):
+        run(opt, ps, 5, skip={(0, 1), (3, 2)})
+    for p, q in zip(ours, theirs):
+        torch.testing.assert_close(p, q, rtol=1e-6, atol=1e-6)
+    assert [a.state[p]["step"] for p in ours] == [5, 4, 4]
+
+
+@pytest.mark.parametrize("source", ["own", "torch"])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_adamw_state_dicts_load(cpu_kernels, source, capturable):
+    first = parameters(0, torch.bfloat16)
+    kw = dict(lr=1e-2, weight_decay=0.1)
+    a = optim.AdamW(first, **kw, master_weights=True, ema_decay=0.9) if source == "own" else torch.optim.AdamW(first, **kw)
+    run(a, first, 3)
+    saved = copy.deepcopy(a.state_dict())
+    second = [torch.nn.Parameter(p.detach().clone()) for p in first]
+    b = optim.AdamW(second, **kw, master_weights=True, ema_decay=0.9, capturable=capturable)
+    b.load_state_dict(saved)
+    if source == "own":
+        assert b.param_groups[0]["capturable"] is False  # a saved group's options are the optimizer's
+        for p, q in zip(first, second):
+            for key in ("exp_avg", "exp_avg_sq", "master", "ema"):
+                assert b.state[q][key].dtype == torch.float32 and torch.equal(a.state[p][key], b.state[q][key])
+        run(a, first, 2, seed=7)
+        run(b, second, 2, seed=7)
+        for p, q in zip(first, second):
+            assert torch.equal(p, q) and b.state[q]["step"] == 5
+    else:
+        run(b, second, 1)
+        assert all(b.state[q]["step"] == 4 for q in second)
+        assert all(b.state[q]["exp_avg"].dtype == torch.float32 for q in second)
+
+
+def test_adamw_capturable_counts_on_the_device_and_round_trips(cpu_kernels):
+    params = parameters(0)
+    a = optim.AdamW(params, lr=torch.tensor(1e-2), capturable=True)
+    run(a, params, 3)
+    counts = {id(a.state[p]["step"]) for p in params}
+    assert len(counts) == 1 and float(a.state[params[0]]["step"]) == 3
+    other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    b = optim.AdamW(other, lr=torch.tensor(1e-2), capturable=True)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    run(a, params, 2, seed=9)
+    run(b, other, 2, seed=9)
+    for p, q in zip(params, other):
+        assert torch.equal(p, q) and float(b.state[q]["step"]) == 5
+
+
+def test_adamw_ema_and_clipping_norm(cpu_kernels):
+    params = parameters(0)
+    a = optim.AdamW(params, lr=1e-2, ema_decay=0.5, max_norm=1.0)
+    before = [p.detach().clone() for p in params]
+    assert all(torch.equal(e, p) for e, p in zip(a.ema_params(), before))
+    run(a, params, 1)
+    want = torch.linalg.vector_norm(torch.cat([p.grad.flatten() for p in params]))
+    torch.testing.assert_close(a.last_grad_norm, want)
+    for e, p, q in zip(a.ema_params(params), params, before):
+        torch.testing.assert_close(e, 0.5 * q + 0.5 * p)
+
+
+def test_adamw_refuses_states_it_does_not_have(cpu_kernels):
+    params = parameters(0)
+    b = torch.optim.AdamW(params, amsgrad=True)
+    run(b, params, 1)
+    with pytest.raises(ValueError, match="amsgrad"):
+        optim.AdamW(params).load_state_dict(b.state_dict())
