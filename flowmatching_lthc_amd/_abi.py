@@ -75,6 +75,9 @@ EXPORTS = (
     "lthc_interface_workspace_bytes",
     "lthc_interface_fwd",
     "lthc_interface_bwd",
+    "lthc_gated_linear_fwd",
+    "lthc_gated_linear_bwd_workspace_bytes",
+    "lthc_gated_linear_bwd",
     "lthc_axial_rope",
     "lthc_adamw_step",
     "lthc_adamw_state_values",
@@ -162,6 +165,8 @@ def load() -> ctypes.CDLL:
         "lthc_block_tail_fwd": [
             vp, vp, vp, vp, ci, vp, ci, vp, ci, vp, vp, i64, vp, vp, vp, i64, i64, i64, ctypes.c_float, vp,
         ],  # fmt: skip
+        "lthc_gated_linear_fwd": [vp, vp, vp, ci, ci, vp, i64, i64, i64, vp],
+        "lthc_gated_linear_bwd": [vp, vp, vp, vp, ci, ci, vp, vp, vp, i64, i64, i64, vp, sz, vp],
         "lthc_axial_rope": [
             vp, vp, pi, i64, vp, vp, pi, i64, ci, vp, ci, pi, vp, pi, i64, ci, ci, i64, i64, i64, vp,
         ],  # fmt: skip
@@ -198,7 +203,7 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name + "_workspace_bytes")
         fn.argtypes = [i64, i64, i64, i64]
         fn.restype = sz
-    for name in ("lthc_gate_add_norm_modulate_bwd", "lthc_gate_residual_bwd", "lthc_linear_weight_grad"):
+    for name in ("lthc_gate_add_norm_modulate_bwd", "lthc_gate_residual_bwd", "lthc_linear_weight_grad", "lthc_gated_linear_bwd"):
         fn = getattr(lib, name + "_workspace_bytes")
         fn.argtypes = [i64, i64, i64]
         fn.restype = sz

@@ -961,6 +961,73 @@ std::tuple<Tensor, Tensor, Tensor> block_tail_cuda(const Tensor& z_, const Tenso
 }
 
 // ---------------------------------------------------------------------------
+// gated linear layer
+// ---------------------------------------------------------------------------
+int act_code(c10::string_view act) {
+  if (act == "silu") return LTHC_ACT_SILU;
+  if (act == "gelu") return LTHC_ACT_GELU;
+  if (act == "gelu_tanh") return LTHC_ACT_GELU_TANH;
+  TORCH_CHECK_VALUE(false, "activation must be silu, gelu or gelu_tanh, got ", act);
+}
+
+bool given(const std::optional<Tensor>& t) { return t.has_value() && t->defined(); }
+
+// F.
+int64_t check_gated(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(0) % 2 == 0 && weight.size(0) > 0 &&
+                        x.size(-1) == weight.size(1),
+                    "x [..., C] and weight [2F, C] expected, got ", shape(x), " and ", shape(weight));
+  TORCH_CHECK_VALUE(x.size(-1) % 8 == 0 && x.size(-1) > 0, "C must be a multiple of 8, got ", x.size(-1));
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "x must be bf16 or fp16, got ",
+                    x.scalar_type());
+  TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() && (!given(bias) || bias->scalar_type() == x.scalar_type()),
+                    "weight and bias must have x's dtype ", x.scalar_type());
+  TORCH_CHECK_VALUE(!given(bias) || has_shape(*bias, {weight.size(0)}), "bias must be [", weight.size(0), "]");
+  on_gpu(x, weight);
+  if (given(bias)) on_gpu(x, *bias);
+  return weight.size(0) / 2;
+}
+
+Tensor gated_linear_cuda(const Tensor& x_, const Tensor& weight, const std::optional<Tensor>& bias, c10::string_view activation) {
+  const int act = act_code(activation);
+  const int64_t f = check_gated(x_, weight, bias);
+  const Tensor x = prep16(x_), w = prep16(weight), b = given(bias) ? bias->contiguous() : Tensor();
+  auto sizes = x.sizes().vec();
+  sizes.back() = f;
+  Tensor y = at::empty(sizes, x.options());
+  const int64_t c = x.size(-1);
+  const Launch l(x);
+  check(lthc_gated_linear_fwd(data(x), data(w), b.defined() ? data(b) : nullptr, code(x), act, data(y), x.numel() / c, c, f,
+                              l.stream),
+        "lthc_gated_linear_fwd");
+  return y;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_linear_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& weight,
+                                                              const std::optional<Tensor>& bias, c10::string_view activation,
+                                                              bool need_x, bool need_weight, bool need_bias) {
+  const int act = act_code(activation);
+  const int64_t f = check_gated(x_, weight, bias), c = x_.size(-1), m = x_.numel() / c;
+  auto sizes = x_.sizes().vec();
+  sizes.back() = f;
+  on_gpu(x_, grad_);
+  check_like(grad_, sizes, "grad");
+  TORCH_CHECK_VALUE(!need_bias || given(bias), "no bias, no gradient of it");
+  const Tensor grad = grad_.to(x_.scalar_type()).contiguous(), x = prep16(x_), w = prep16(weight);
+  const Tensor b = given(bias) ? bias->contiguous() : Tensor();
+  Tensor gx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor gw = at::empty({need_weight || need_bias ? 2 * f : 0, c}, x.options());
+  Tensor gb = at::empty({need_bias ? 2 * f : 0}, x.options());
+  const Tensor ws = workspace(lthc_gated_linear_bwd_workspace_bytes(m, c, f), x);
+  const Launch l(x);
+  check(lthc_gated_linear_bwd(data(grad), data(x), data(w), b.defined() ? data(b) : nullptr, code(x), act,
+                              need_x ? data(gx) : nullptr, need_weight || need_bias ? data(gw) : nullptr,
+                              need_bias ? data(gb) : nullptr, m, c, f, data(ws), ws.numel(), l.stream),
+        "lthc_gated_linear_bwd");
+  return {gx, gw, gb};
+}
+
+// ---------------------------------------------------------------------------
 // rotary positions with several axes
 // ---------------------------------------------------------------------------
 int position_code(const Tensor& t) {
@@ -1278,6 +1345,12 @@ LTHC_REPLAY(replay_qk, "qk_norm_rope")
 LTHC_REPLAY(replay_attention, "qk_norm_rope_attention")
 LTHC_REPLAY(replay_swiglu, "swiglu")
 LTHC_REPLAY(replay_ganm, "gate_add_norm_modulate")
+LTHC_OP(op_gated, "gated_linear", Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, c10::string_view))
+LTHC_OP(op_gated_backward, "gated_linear_backward",
+        std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+                                           c10::string_view, bool, bool, bool))
+LTHC_OP(replay_gated, "gated_linear_backward_replay",
+        std::vector<Tensor>(const Tensor&, TensorList, c10::string_view, bool))
 LTHC_OP(op_axial_rope, "axial_rope",
         std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, at::IntArrayRef, bool, bool))
 LTHC_OP(op_linear_weight_grad, "linear_weight_grad", std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, bool))
@@ -1828,6 +1901,33 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
+// The gated linear layer: one backward op for the gradients that are asked for.  Traced, or where a graph of the backward
+// is built, the eager sequence is differentiated.
+struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+                        c10::string_view activation) {
+    BelowAutograd below;
+    ctx->save_for_backward({x, weight, given(bias) ? *bias : Tensor()});
+    ctx->saved_data["activation"] = std::string(activation);
+    return op_gated().call(x, weight, bias, activation);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    const std::string activation = ctx->saved_data["activation"].toStringRef();
+    const bool biased = s[2].defined(), graph = at::GradMode::is_enabled();
+    if (graph || traced(s[0])) {
+      std::vector<Tensor> args{s[0], s[1]};
+      if (biased) args.push_back(s[2]);
+      return wanted(ctx, replay_gated().call(grads[0], args, activation, graph), 4);
+    }
+    DetachedScope scope;
+    const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), biased && ctx->needs_input_grad(2)};
+    auto [gx, gw, gb] = op_gated_backward().call(grads[0], s[0], s[1], biased ? std::optional<Tensor>(s[2]) : std::nullopt,
+                                                 activation, need[0], need[1], need[2]);
+    return {need[0] ? gx : Tensor(), need[1] ? gw : Tensor(), need[2] ? gb : Tensor(), Tensor()};
+  }
+};
+
 // The gradient of a rotation is the rotation by the negative angle.  A side whose gradient is not asked for takes part
 // with no heads.
 struct AxialRopeFn : torch::autograd::Function<AxialRopeFn> {
@@ -1968,6 +2068,20 @@ Tensor gres_autograd(const Tensor& d, const Tensor& gate, const Tensor& m) {
   return op_gres().call(d, gate, m);
 }
 
+Tensor gated_autograd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, c10::string_view activation) {
+  if (recording(x, weight) || (given(bias) && recording(*bias))) return GatedLinearFn::apply(x, weight, bias, activation);
+  BelowAutograd below;
+  return op_gated().call(x, weight, bias, activation);
+}
+
+// Under autocast the operands take its dtype, as linear's do.
+Tensor gated_autocast(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, c10::string_view activation) {
+  c10::impl::ExcludeDispatchKeyGuard off(c10::DispatchKey::AutocastCUDA);
+  const auto dt = at::autocast::get_autocast_dtype(at::kCUDA);
+  const auto cast = [dt](const Tensor& t) { return at::autocast::cached_cast(dt, t, at::kCUDA); };
+  return op_gated().call(cast(x), cast(weight), given(bias) ? std::optional<Tensor>(cast(*bias)) : std::nullopt, activation);
+}
+
 std::tuple<Tensor, Tensor> axial_rope_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
                                                at::IntArrayRef sections, bool interleaved, bool inverse) {
   TORCH_CHECK_VALUE(!recording(positions, inv_freq), "axial_rope gives no gradient of positions or inv_freq");
@@ -2052,6 +2166,8 @@ TORCH_LIBRARY_IMPL(jit_thc, CUDA, m) {
   m.impl("gate_residual_backward", gate_residual_backward_cuda);
   m.impl("linear_weight_grad", linear_weight_grad_cuda);
   m.impl("block_tail", block_tail_cuda);
+  m.impl("gated_linear", gated_linear_cuda);
+  m.impl("gated_linear_backward", gated_linear_backward_cuda);
   m.impl("axial_rope", axial_rope_cuda);
   m.impl("adamw_step", adamw_step_cuda);
   m.impl("adamw_state_values", adamw_state_values_cuda);
@@ -2078,9 +2194,11 @@ static void autograd_kernels(torch::Library& m) {
   m.impl("swiglu", swiglu_autograd);
   m.impl("gate_add_norm_modulate", ganm_autograd);
   m.impl("gate_residual", gres_autograd);
+  m.impl("gated_linear", gated_autograd);
   m.impl("axial_rope", axial_rope_autograd);
 }
 
+TORCH_LIBRARY_IMPL(jit_thc, AutocastCUDA, m) { m.impl("gated_linear", gated_autocast); }
 TORCH_LIBRARY_IMPL(jit_thc, AutogradCUDA, m) { autograd_kernels(m); }
 TORCH_LIBRARY_IMPL(jit_thc, AutogradMeta, m) { autograd_kernels(m); }
 TORCH_LIBRARY_IMPL(jit_thc, AutogradCPU, m) { autograd_kernels(m); }

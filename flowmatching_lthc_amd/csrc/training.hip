@@ -8,3 +8,5 @@
 #include "axial_rope.inc"
 // AdamW, the norm of all gradients.
 #include "adamw.inc"
+// The gated linear layer and its backward.
+#include "gated_linear.inc"

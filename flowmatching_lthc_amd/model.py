@@ -348,8 +348,29 @@ class SwiGLUFFN(nn.Module):
         self.w12 = CastLinear(dim, 2 * hidden, bias=bias)
         self.w3 = CastLinear(hidden, dim, bias=bias)
         self.ffn_dropout = nn.Dropout(drop)
+        # w12, silu and the product as one HIP pass (jit_thc::gated_linear) where it applies.  Off: the eager sequence
+        # rounds the projections to the activation dtype, the fused pass does not.
+        self.fused_projections = False
+
+    def _fused_act(self, x: torch.Tensor) -> torch.Tensor | None:
+        """The gated hidden activations from jit_thc::gated_linear, or None where it is switched off or does not take them."""
+        cast = self.w12.__dict__.get("_cast")
+        w, b = cast if cast is not None else (self.w12.weight, self.w12.bias)
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        if not (
+            self.fused_projections
+            and x.is_cuda
+            and dt in (torch.bfloat16, torch.float16)
+            and (torch.is_autocast_enabled("cuda") or w.dtype == dt and (b is None or b.dtype == dt))
+            and x.shape[-1] % 8 == 0
+        ):
+            return None
+        return ops_branch.gated_linear(x, w, b)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        act = self._fused_act(x)
+        if act is not None:
+            return self.w3(self.ffn_dropout(act))
         h = self.w12(x)
         if h.is_cuda and h.dtype in (torch.bfloat16, torch.float16, torch.float32) and h.shape[-1] % 16 == 0:
             act = ops_branch.swiglu(h)  # silu(gate) * value in one HIP pass, eager roundings

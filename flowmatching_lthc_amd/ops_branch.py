@@ -26,6 +26,8 @@ activation dtype), registered as a ``jit_thc`` custom op:
 
 Two more have no eager sequence in the reference's branch:
 
+* ``jit_thc::gated_linear``: a linear layer's two halves, an activation and their product (``w12`` and ``swiglu`` of
+  SwiGLUFFN) as one matrix-core pass, without the eager sequence's roundings in between;
 * ``jit_thc::axial_rope``: rotary positions with several axes on q and k, for token maps that
   VisionRotaryEmbeddingFast's square grid does not describe (frames, oblong maps, single tokens).
 
@@ -370,6 +372,65 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor | None:
     if dt not in (torch.bfloat16, torch.float16) or weight.device != x.device:
         return None
     return torch.ops.jit_thc.linear(x, weight, bias)
+
+
+# ---------------------------------------------------------------------------
+# gated linear layer: both projections of a gated feed-forward, the activation and the product
+# ---------------------------------------------------------------------------
+ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh")}
+
+
+def gated_linear_eager(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str = "silu") -> Tensor:
+    """gated_linear's function from F.linear, its projections and their product in fp32, rounded once."""
+    h = F.linear(x.float(), weight.float(), None if bias is None else bias.float())
+    g, u = h.chunk(2, dim=-1)
+    return (ACTIVATIONS[activation](g) * u).to(x.dtype)
+
+
+@torch.library.custom_op("jit_thc::gated_linear", mutates_args=())
+def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str = "silu") -> Tensor:
+    """act(x Wg^T + bg) * (x Wu^T + bu) in x's dtype for x [..., C], weight [2F, C] = (Wg, Wu), bias [2F] = (bg, bu) or
+    none, activation silu, gelu or gelu_tanh: the w12 projection and gate of SwiGLUFFN in one matrix-core pass, the
+    projections in fp32 up to the one rounding of the result.
+
+    bf16 or fp16 (under autocast, its dtype), C a multiple of 8, any F.  The backward recomputes the projections; a second
+    derivative goes through gated_linear_eager."""
+    _refuse(x)
+
+
+@_fake(gated_linear)
+def _(x, weight, bias=None, activation="silu"):
+    return x.new_empty((*x.shape[:-1], weight.shape[0] // 2))
+
+
+@torch.library.custom_op("jit_thc::gated_linear_backward", mutates_args=())
+def gated_linear_backward(
+    grad: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, activation: str, need_x: bool, need_weight: bool, need_bias: bool
+) -> tuple[Tensor, Tensor, Tensor]:
+    """Gradients of gated_linear's x, weight and bias for the output gradient [..., F], in x's dtype; one that is not needed
+    is empty (the weight's comes with the bias's)."""
+    _refuse(x)
+
+
+@_fake(gated_linear_backward)
+def _(grad, x, weight, bias, activation, need_x, need_weight, need_bias):
+    n = weight.shape[0]
+    gx = x.new_empty(x.shape if need_x else (0,))
+    return gx, x.new_empty((n if need_weight or need_bias else 0, weight.shape[1])), x.new_empty((n if need_bias else 0,))
+
+
+def _gated_linear_replay(grad: Tensor, args: list[Tensor], activation: str, graph: bool) -> list[Tensor]:
+    with torch.enable_grad():
+        if not graph:
+            args = [t.detach().requires_grad_() for t in args]
+        else:  # leaves that ask for no gradient take part in the differentiation all the same
+            args = [t if t.requires_grad else t.detach().requires_grad_() for t in args]
+        out = gated_linear_eager(args[0], args[1], args[2] if len(args) > 2 else None, activation)
+        return list(torch.autograd.grad(out, args, grad, create_graph=graph))
+
+
+torch.library.define("jit_thc::gated_linear_backward_replay", "(Tensor grad, Tensor[] args, str activation, bool graph) -> Tensor[]")
+torch.library.impl("jit_thc::gated_linear_backward_replay", "CompositeImplicitAutograd")(_gated_linear_replay)
 
 
 # ---------------------------------------------------------------------------

@@ -569,6 +569,27 @@ int lthc_interface_bwd(const void* gx, const void* const* gz, int x_dtype, const
                        size_t workspace_bytes, void* stream);
 
 /*
+ * GATED LINEAR LAYER (no reference op: the w12 projection and silu(x1) * x2 of
+ * SwiGLUFFN.forward, local_thc.py:259-269).  For x [M, C], weight [2F, C] =
+ * (Wg, Wu) and bias [2F] (NULL: none), all x_dtype (bf16 or fp16):
+ *   y[m, f] = act(x[m] . Wg[f] + bg[f]) * (x[m] . Wu[f] + bu[f])
+ * in fp32, rounded once.  act: LTHC_ACT_SILU, _GELU (erf), _GELU_TANH.  C a
+ * multiple of 8; any F and M; x and weight 16-byte aligned, 4 F C < 2^31 - 2^24.
+ * Backward for dy [M, F]: dx [M, C], dw [2F, C] and db [2F], each NULL where it is
+ * not wanted (db comes with dw).  The projections are recomputed; their gradients
+ * are rounded to x_dtype once, where they enter the products.
+ */
+#define LTHC_ACT_SILU 0
+#define LTHC_ACT_GELU 1
+#define LTHC_ACT_GELU_TANH 2
+int lthc_gated_linear_fwd(const void* x, const void* weight, const void* bias, int x_dtype, int act, void* y, int64_t M,
+                          int64_t C, int64_t F, void* stream);
+size_t lthc_gated_linear_bwd_workspace_bytes(int64_t M, int64_t C, int64_t F);
+int lthc_gated_linear_bwd(const void* dy, const void* x, const void* weight, const void* bias, int x_dtype, int act, void* dx,
+                          void* dw, void* db, int64_t M, int64_t C, int64_t F, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
  * ROTARY POSITIONS WITH SEVERAL AXES (no reference op: VisionRotaryEmbeddingFast,
  * jit_shared_adaln.py:33-59, has two axes and a table of one square grid).  For
  * q and k, B x N tokens of q_heads and k_heads heads of D channels (x_dtype):

@@ -243,3 +243,68 @@ def test_adamw_refuses_states_it_does_not_have(cpu_kernels):
     run(b, params, 1)
     with pytest.raises(ValueError, match="amsgrad"):
         optim.AdamW(params).load_state_dict(b.state_dict())
+
+
+# ---------------------------------------------------------------------------
+# gated linear layer
+# ---------------------------------------------------------------------------
+def gated(M=4, C=16, F=6, x=4096, w=4096, b=4096, y=4096, dtype=_abi.BF16, act=0):
+    return err(_abi.load().lthc_gated_linear_fwd(x, w, b, dtype, act, y, M, C, F, None))
+
+
+def test_gated_linear_refusals_of_the_c_entries():
+    for kw, text in (
+        (dict(C=12), "multiple of 8"),
+        (dict(C=0), "positive"),
+        (dict(F=0), "positive"),
+        (dict(M=-1), "positive"),
+        (dict(dtype=_abi.F32), "bf16 or fp16"),
+        (dict(act=3), "activation"),
+        (dict(x=None), "aligned"),
+        (dict(w=4104), "aligned"),
+        (dict(b=4097), "bias"),
+        (dict(y=None), "y is NULL"),
+        (dict(C=1 << 16, F=1 << 14), "range"),
+    ):
+        rc, msg = gated(**kw)
+        assert rc in (_abi.ERR_INVALID, _abi.ERR_UNSUPPORTED) and text in msg, (kw, rc, msg)
+    assert gated(M=0, x=None, w=None, y=None)[0] == _abi.OK
+    lib = _abi.load()
+    need = lib.lthc_gated_linear_bwd_workspace_bytes(100, 16, 6)
+    assert need >= 100 * 16 * 2 + 16 * 16 * 2 and lib.lthc_gated_linear_bwd_workspace_bytes(0, 16, 6) == 0
+    for ws, size, text, db, dw in (
+        (4096, need - 1, "workspace", 4096, 4096),
+        (4096 + 16, need, "workspace", 4096, 4096),
+        (None, need, "workspace", 4096, 4096),
+        (4096, need, "db comes", 4096, None),
+        (4096, need, "dw must", 4096, 4104),
+        (4096, need, "db must", 4098, 4096),
+    ):
+        rc, msg = err(lib.lthc_gated_linear_bwd(4096, 4096, 4096, None, _abi.BF16, 0, 4096, dw, db, 100, 16, 6, ws, size, None))
+        assert rc == _abi.ERR_INVALID and text in msg, (msg, text)
+
+
+def test_gated_linear_refuses_cpu_tensors_and_predicts_its_outputs():
+    x, w = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(6, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        OB.gated_linear(x, w)
+    y = OB.gated_linear(meta(2, 5, 8, dtype=torch.bfloat16), meta(6, 8, dtype=torch.bfloat16))
+    assert y.shape == (2, 5, 3) and y.dtype == torch.bfloat16
+    gx, gw, gb = OB.gated_linear_backward(y, meta(2, 5, 8), meta(6, 8), None, "silu", True, False, False)
+    assert gx.shape == (2, 5, 8) and gw.shape == (0, 8) and gb.shape == (0,)
+
+
+def test_gated_linear_eager_is_swiglu_of_the_projections():
+    x, w, b = torch.randn(4, 8), torch.randn(6, 8), torch.randn(6)
+    want = OB.swiglu_eager(torch.nn.functional.linear(x, w, b))
+    torch.testing.assert_close(OB.gated_linear_eager(x, w, b), want)
+
+
+def test_gated_linear_stays_off_in_the_model_by_default():
+    from flowmatching_lthc_amd.model import SwiGLUFFN
+
+    ffn = SwiGLUFFN(16, 48)
+    assert ffn.fused_projections is False
+    x = torch.randn(3, 16)
+    ffn.fused_projections = True  # CPU tensors keep the eager sequence
+    torch.testing.assert_close(ffn(x), ffn.w3(OB.swiglu_eager(ffn.w12(x))))
