@@ -576,7 +576,7 @@ int lthc_interface_bwd(const void* gx, const void* const* gz, int x_dtype, const
  * in fp32, rounded once.  act: LTHC_ACT_SILU, _GELU (erf), _GELU_TANH.  C a
  * multiple of 8; any F and M; x and weight 16-byte aligned, 4 F C < 2^31 - 2^24.
  * Backward for dy [M, F]: dx [M, C], dw [2F, C] and db [2F], each NULL where it is
- * not wanted (db comes with dw).  The projections are recomputed; their gradients
+ * not wanted.  The projections are recomputed; their gradients
  * are rounded to x_dtype once, where they enter the products.
  */
 #define LTHC_ACT_SILU 0

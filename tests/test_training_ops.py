@@ -276,7 +276,6 @@ def test_gated_linear_refusals_of_the_c_entries():
         (4096, need - 1, "workspace", 4096, 4096),
         (4096 + 16, need, "workspace", 4096, 4096),
         (None, need, "workspace", 4096, 4096),
-        (4096, need, "db comes", 4096, None),
         (4096, need, "dw must", 4096, 4104),
         (4096, need, "db must", 4098, 4096),
     ):
