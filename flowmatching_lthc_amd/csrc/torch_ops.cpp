@@ -1131,18 +1131,32 @@ void same_layout(TensorList ts, TensorList params, const char* name) {
                       ", got ", ts[i].sizes(), ", ", ts[i].strides());
 }
 
-// Every tensor that the step writes has its memory for itself (the kernels' blocks run in no order).
-void no_overlap(std::initializer_list<TensorList> lists) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+// Every tensor that the step writes has its memory for itself (the kernels' blocks run in no order); what it only reads may
+// be there twice.
+void no_overlap(std::initializer_list<TensorList> lists, std::initializer_list<TensorList> read) {
+  using Span = std::pair<uintptr_t, uintptr_t>;
+  auto span = [](const Tensor& t) {
+    const auto at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    return Span(at, at + t.numel() * t.element_size());
+  };
+  std::vector<Span> spans;
+  size_t count = 0;
+  for (const TensorList l : lists) count += l.size();
+  spans.reserve(count);
   for (const TensorList l : lists)
     for (const Tensor& t : l)
-      if (t.numel() > 0) {
-        const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
-        spans.emplace_back(at, at + t.numel() * t.element_size());
-      }
+      if (t.numel() > 0) spans.push_back(span(t));
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
     TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "tensors that the step writes overlap (the same tensor twice?)");
+  for (const TensorList l : read)
+    for (const Tensor& t : l) {
+      if (t.numel() == 0) continue;
+      const Span s = span(t);
+      const auto next = std::lower_bound(spans.begin(), spans.end(), Span(s.second, 0));  // the first that begins past it
+      TORCH_CHECK_VALUE(next == spans.begin() || std::prev(next)->second <= s.first,
+                        "a tensor that the step reads overlaps one that it writes");
+    }
 }
 
 void written(TensorList ts) {
@@ -1160,6 +1174,7 @@ const float* device_scalar(const std::optional<Tensor>& t, const Tensor& like, c
 
 std::vector<int64_t> numels(TensorList ts) {
   std::vector<int64_t> n;
+  n.reserve(ts.size());
   for (const Tensor& t : ts) n.push_back(t.numel());
   return n;
 }
@@ -1204,6 +1219,7 @@ void adamw_step_cuda(TensorList params, TensorList grads_, TensorList avgs, Tens
     same_layout(emas, params, "ema");
   }
   std::vector<Tensor> grads;
+  grads.reserve(params.size());
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor &p = params[i], &g = grads_[i];
     TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "parameter ", i, " must fill its memory (strides ", p.strides(), ")");
@@ -1211,7 +1227,10 @@ void adamw_step_cuda(TensorList params, TensorList grads_, TensorList avgs, Tens
     const bool as_is = g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous());
     grads.push_back(as_is ? g : at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g));
   }
-  no_overlap({params, avgs, sqs, scales, masters, emas});
+  std::vector<Tensor> scalars;
+  for (const auto* t : {&device_step, &device_lr, &grad_norm})
+    if (t->has_value() && (*t)->defined()) scalars.push_back(**t);
+  no_overlap({params, avgs, sqs, scales, masters, emas}, {grads, scalars});
   const float* dstep = device_scalar(device_step, first, "step");
   const float* dlr = device_scalar(device_lr, first, "lr");
   const float* norm = device_scalar(grad_norm, first, "grad_norm");
@@ -1220,6 +1239,7 @@ void adamw_step_cuda(TensorList params, TensorList grads_, TensorList avgs, Tens
   const auto g = pointers(grads);
   auto floats = [](TensorList ts) {
     std::vector<float*> out;
+    out.reserve(ts.size());
     for (const Tensor& t : ts) out.push_back(static_cast<float*>(t.data_ptr()));
     return out;
   };
@@ -1262,6 +1282,7 @@ Tensor grad_norm_cuda(TensorList grads_) {
   TORCH_CHECK_VALUE(!grads_.empty(), "grad_norm of no tensors");
   check_many(grads_, "grads", grads_[0], grads_.size(), {at::kFloat, at::kBFloat16, at::kHalf});
   std::vector<Tensor> grads;
+  grads.reserve(grads_.size());
   for (const Tensor& g : grads_) grads.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
   const auto n = numels(grads);
   const auto g = pointers(grads);
@@ -2196,6 +2217,7 @@ static void autograd_kernels(torch::Library& m) {
   m.impl("gate_residual", gres_autograd);
   m.impl("gated_linear", gated_autograd);
   m.impl("axial_rope", axial_rope_autograd);
+  for (const char* name : {"adamw_step", "adamw_state_values", "grad_norm"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(jit_thc, AutocastCUDA, m) { m.impl("gated_linear", gated_autocast); }

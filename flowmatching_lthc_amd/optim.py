@@ -53,6 +53,10 @@ _define(
 _define("grad_norm", "(Tensor[] grads) -> Tensor", lambda grads: grads[0].new_empty((), dtype=torch.float32))
 
 
+def _list(ts: Sequence[Tensor]) -> list[Tensor]:
+    return ts if isinstance(ts, list) else list(ts)
+
+
 @torch.no_grad()
 def adamw_step(
     params: Sequence[Tensor],
@@ -78,12 +82,13 @@ def adamw_step(
     layout, or, with `scales` (fp32 [2, runs of 256]), contiguous int8 and uint8 codes.  masters: fp32 copies of 16-bit
     parameters, which take the step and are rounded into them.  emas: fp32 moving averages.  grad_norm: the norm of all
     gradients (one fp32 on the device); they are scaled by min(1, max_norm / (grad_norm + 1e-6)), and where it is not finite
-    nothing is changed.  step and lr may be one fp32 on the device, which a captured graph reads anew on each replay."""
+    nothing is changed.  What the step writes lies in memory of its own; a gradient may be there twice.  step and lr may be
+    one fp32 on the device, which a captured graph reads anew on each replay."""
     if not len(params):
         return
     on_device = isinstance(step, Tensor), isinstance(lr, Tensor)
     torch.ops.jit_thc.adamw_step(
-        list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(scales), list(masters), list(emas),
+        _list(params), _list(grads), _list(exp_avgs), _list(exp_avg_sqs), _list(scales), _list(masters), _list(emas),
         1.0 if on_device[0] else float(step), 0.0 if on_device[1] else float(lr), betas[0], betas[1], eps, weight_decay, ema_decay,
         step if on_device[0] else None, lr if on_device[1] else None, grad_norm, max_norm,
     )  # fmt: skip

@@ -407,3 +407,25 @@ def test_optimizer_in_bf16_with_master_weights_and_its_checkpoint(bits, tmp_path
             assert torch.equal(torch.as_tensor(value), torch.as_tensor(opt2.state[q][key])), key
     for e, p in zip(opt.ema_params(a.parameters()), a.parameters()):
         assert e.dtype == F32 and e.shape == p.shape
+
+
+def test_gradients_may_be_there_twice_but_not_in_written_memory():
+    print("case adamw gradients shared", flush=True)
+    s = State([(300,), (300,)])
+    t = State([(300,), (300,)])
+    kw = dict(lr=1e-2, step=1)
+    optim.adamw_step(s.p, [s.g[0], s.g[0]], s.m, s.v, **kw)
+    optim.adamw_step(t.p, [s.g[0], s.g[0].clone()], t.m, t.v, **kw)
+    for a, c in zip((*s.p, *s.m, *s.v), (*t.p, *t.m, *t.v)):
+        assert torch.equal(a, c)
+    whole = torch.zeros(700, device=DEV)
+    for g in (s.p[1], s.m[1]):
+        with pytest.raises(ValueError, match="overlaps"):
+            optim.adamw_step(s.p, [s.g[0], g], s.m, s.v, **kw)
+    with pytest.raises(ValueError, match="overlaps"):
+        optim.adamw_step([whole[:300]], [whole[299:599]], s.m[:1], s.v[:1], **kw)
+    optim.adamw_step([whole[:300]], [whole[300:600]], s.m[:1], s.v[:1], **kw)  # side by side
+    with pytest.raises(ValueError, match="overlaps"):
+        optim.adamw_step([whole[:300]], s.g[:1], s.m[:1], s.v[:1], lr=1e-2, step=whole[:1])
+    with pytest.raises(ValueError, match="overlaps"):
+        optim.adamw_step([whole[:300]], s.g[:1], s.m[:1], s.v[:1], lr=1e-2, step=1, grad_norm=whole[299:300], max_norm=1.0)
