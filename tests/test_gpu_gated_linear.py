@@ -318,3 +318,20 @@ def test_the_models_feed_forward_with_fused_projections():
 def F_ref(ffn, x):
     g, u = ffn.w12(x).chunk(2, -1)
     return ffn.w3(OB.swiglu(torch.cat([g, u], -1)))
+
+
+@pytest.mark.parametrize("M", [5, 128, 300])
+def test_an_infinite_bias_reaches_only_its_own_sums(M):
+    """Rows past the last one add nothing to the bias gradients, whatever the bias makes of them."""
+    print("case gated_linear infinite bias", M, flush=True)
+    C, Fh = 16, 70
+    x, w = randn((M, C), 0, torch.bfloat16).abs(), randn((2 * Fh, C), 1, torch.bfloat16).abs()
+    b = torch.zeros(2 * Fh, device=DEV, dtype=torch.bfloat16)
+    b[Fh + 3] = math.inf  # an up projection: its gate's gradient is dy inf act'(g), act'(g) > 0
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    dy = randn((M, Fh), 2, torch.bfloat16).abs() + 0.5
+    _, dw, db = torch.autograd.grad(OB.gated_linear(x, w, b), [x, w, b], dy)
+    assert float(db[3]) == math.inf
+    rest = torch.ones(2 * Fh, dtype=torch.bool, device=DEV)
+    rest[3] = False
+    assert bool(db[rest].isfinite().all()) and bool(dw[rest].isfinite().all())
