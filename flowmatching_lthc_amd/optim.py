@@ -109,6 +109,10 @@ def grad_norm(grads: Sequence[Tensor]) -> Tensor:
     return torch.ops.jit_thc.grad_norm(list(grads))
 
 
+def _capturing(t: Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update on the operators above.  What it has besides:
 
@@ -119,8 +123,9 @@ class AdamW(torch.optim.Optimizer):
       parameter's first step;
     * ``max_norm``: clipping by the norm of all gradients, which ``last_grad_norm`` keeps on the device; a step whose norm is
       not finite changes no tensor (it is counted);
-    * ``capturable``: step counts on the device, one for all parameters that step together from their first step on, and a
-      learning rate that may be a tensor there, so that a captured step can be replayed.
+    * ``capturable``: step counts on the device, one for all parameters that have taken the same steps, and a learning rate
+      that may be a tensor there, so that a captured step can be replayed.  Its states are laid out by a step outside the
+      capture, with the same parameters having gradients; other captured steps are refused.
 
     The state has torch.optim.AdamW's names (``step``, ``exp_avg``, ``exp_avg_sq``; the codes' ``scales``), and that
     optimizer's ``state_dict`` loads."""
@@ -165,6 +170,11 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def _init_state(self, p: Tensor, group: dict) -> dict:
         state = self.state[p]
+        missing = "exp_avg" not in state or (
+            group["master_weights"] and p.dtype != torch.float32 and "master" not in state
+        ) or (group["ema_decay"] is not None and "ema" not in state)  # fmt: skip
+        if missing and _capturing(p):
+            raise RuntimeError("a captured AdamW step needs its states: take one step outside the capture first")
         if "exp_avg" not in state:
             if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:
                 state["exp_avg"] = torch.zeros(p.numel(), device=p.device, dtype=torch.int8)
@@ -188,6 +198,28 @@ class AdamW(torch.optim.Optimizer):
         for s in states:
             s["step"] = have
         return have
+
+    def _split_counts(self) -> None:
+        """Parameters that take a step which others of their shared count do not take get a count of their own."""
+        for group in self.param_groups:
+            if not group["capturable"]:
+                continue
+            stepping: dict[int, list[dict]] = {}
+            resting: set[int] = set()
+            for p in group["params"]:
+                state = self.state.get(p, {})
+                if isinstance(state.get("step"), Tensor):
+                    if p.grad is None:
+                        resting.add(id(state["step"]))
+                    else:
+                        stepping.setdefault(id(state["step"]), []).append(state)
+            for at, states in stepping.items():
+                if at in resting:
+                    if _capturing(states[0]["exp_avg"]):
+                        raise RuntimeError("a captured AdamW step needs the same gradients as the step outside the capture")
+                    own = states[0]["step"].clone()
+                    for state in states:
+                        state["step"] = own
 
     def ema_params(self, params: Iterable[Tensor] | None = None) -> list[Tensor]:
         """The moving averages of `params` (the optimizer's own, in their order), in `params`' shapes: what
@@ -241,6 +273,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._split_counts()
         calls: dict = {}  # one call for each set of tensors that share types, device, state width and step count
         for group in self.param_groups:
             for p in group["params"]:
@@ -249,6 +282,8 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if g.is_sparse:
                     raise ValueError("AdamW takes no sparse gradients")
+                if not group["capturable"] and _capturing(p):
+                    raise RuntimeError("a captured AdamW step needs capturable=True")
                 state = self._init_state(p, group)
                 step = state["step"]
                 key = (id(group), p.device, p.dtype, g.dtype, "scales" in state, id(step) if isinstance(step, Tensor) else step)

@@ -307,3 +307,42 @@ def test_gated_linear_stays_off_in_the_model_by_default():
     x = torch.randn(3, 16)
     ffn.fused_projections = True  # CPU tensors keep the eager sequence
     torch.testing.assert_close(ffn(x), ffn.w3(OB.swiglu_eager(ffn.w12(x))))
+
+
+def test_adamw_capturable_counts_part_where_steps_part(cpu_kernels):
+    """A parameter without a gradient in a step keeps its count, as without capturable."""
+    ours, plain = parameters(0), parameters(0)
+    a = optim.AdamW(ours, lr=1e-2, capturable=True)
+    b = optim.AdamW(plain, lr=1e-2)
+    skip = {(1, 0), (2, 0), (3, 2)}
+    run(a, ours, 5, skip=skip)
+    run(b, plain, 5, skip=skip)
+    for p, q in zip(ours, plain):
+        assert float(a.state[p]["step"]) == b.state[q]["step"]
+        assert torch.equal(p, q)
+    assert [b.state[q]["step"] for q in plain] == [3, 5, 4]
+
+
+def test_adamw_refuses_captures_that_would_not_replay(cpu_kernels, monkeypatch):
+    params = parameters(0)
+    a = optim.AdamW(params, lr=1e-2, capturable=True)
+    b = optim.AdamW(params, lr=1e-2)
+    c = optim.AdamW(params, lr=1e-2, capturable=True, ema_decay=0.9)
+    run(a, params, 1)
+    run(b, params, 1)
+    before = [p.detach().clone() for p in params]
+    monkeypatch.setattr(optim, "_capturing", lambda t: True)
+    run(a, params, 1)  # laid out before: as it should be
+    for opt, skip, text in ((b, (), "capturable"), (c, (), "outside the capture"), (a, {(0, 1)}, "same gradients")):
+        now = [p.detach().clone() for p in params]
+        with pytest.raises(RuntimeError, match=text):
+            run(opt, params, 1, skip=skip)
+        assert all(torch.equal(p, q) for p, q in zip(params, now))
+    assert not all(torch.equal(p, q) for p, q in zip(params, before))
+
+
+def test_gated_linear_workspace_of_sizes_out_of_range():
+    query = _abi.load().lthc_gated_linear_bwd_workspace_bytes
+    for sizes in ((0, 8, 8), (8, -8, 8), (1 << 40, 8, 8), (8, 1 << 40, 8), (8, 8, 1 << 40), (8, 1 << 19, 1 << 19), (-1, 1 << 62, 1 << 62)):
+        assert query(*sizes) == 0, sizes
+    assert query(8, 8, 8) > 0
