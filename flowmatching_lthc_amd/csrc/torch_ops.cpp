@@ -1016,12 +1016,12 @@ std::tuple<Tensor, Tensor, Tensor> gated_linear_backward_cuda(const Tensor& grad
   const Tensor grad = grad_.to(x_.scalar_type()).contiguous(), x = prep16(x_), w = prep16(weight);
   const Tensor b = given(bias) ? bias->contiguous() : Tensor();
   Tensor gx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  Tensor gw = at::empty({need_weight || need_bias ? 2 * f : 0, c}, x.options());
+  Tensor gw = at::empty({need_weight ? 2 * f : 0, c}, x.options());
   Tensor gb = at::empty({need_bias ? 2 * f : 0}, x.options());
   const Tensor ws = workspace(lthc_gated_linear_bwd_workspace_bytes(m, c, f), x);
   const Launch l(x);
   check(lthc_gated_linear_bwd(data(grad), data(x), data(w), b.defined() ? data(b) : nullptr, code(x), act,
-                              need_x ? data(gx) : nullptr, need_weight || need_bias ? data(gw) : nullptr,
+                              need_x ? data(gx) : nullptr, need_weight ? data(gw) : nullptr,
                               need_bias ? data(gb) : nullptr, m, c, f, data(ws), ws.numel(), l.stream),
         "lthc_gated_linear_bwd");
   return {gx, gw, gb};

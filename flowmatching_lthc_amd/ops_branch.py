@@ -408,7 +408,7 @@ def gated_linear_backward(
     grad: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, activation: str, need_x: bool, need_weight: bool, need_bias: bool
 ) -> tuple[Tensor, Tensor, Tensor]:
     """Gradients of gated_linear's x, weight and bias for the output gradient [..., F], in x's dtype; one that is not needed
-    is empty (the weight's comes with the bias's)."""
+    is empty."""
     _refuse(x)
 
 
@@ -416,7 +416,7 @@ def gated_linear_backward(
 def _(grad, x, weight, bias, activation, need_x, need_weight, need_bias):
     n = weight.shape[0]
     gx = x.new_empty(x.shape if need_x else (0,))
-    return gx, x.new_empty((n if need_weight or need_bias else 0, weight.shape[1])), x.new_empty((n if need_bias else 0,))
+    return gx, x.new_empty((n if need_weight else 0, weight.shape[1])), x.new_empty((n if need_bias else 0,))
 
 
 def _gated_linear_replay(grad: Tensor, args: list[Tensor], activation: str, graph: bool) -> list[Tensor]:

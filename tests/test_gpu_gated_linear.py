@@ -335,3 +335,15 @@ def test_an_infinite_bias_reaches_only_its_own_sums(M):
     rest = torch.ones(2 * Fh, dtype=torch.bool, device=DEV)
     rest[3] = False
     assert bool(db[rest].isfinite().all()) and bool(dw[rest].isfinite().all())
+
+
+@pytest.mark.parametrize("M", [3, 700])
+def test_the_backward_op_computes_what_is_needed(M):
+    print("case gated_linear needs", M, flush=True)
+    x, w, b = operands(M, 72, 50, torch.float16)
+    dy = randn((M, 50), 4, torch.float16)
+    full = OB.gated_linear_backward(dy, x, w, b, "gelu", True, True, True)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True)):
+        got = OB.gated_linear_backward(dy, x, w, b, "gelu", *need)
+        for n, g, c, t in zip(need, got, full, torch.ops.jit_thc.gated_linear_backward(*(t.to("meta") for t in (dy, x, w, b)), "gelu", *need)):
+            assert g.shape == t.shape and (torch.equal(g, c) if n else g.numel() == 0)
