@@ -354,12 +354,13 @@ class SwiGLUFFN(nn.Module):
 
     def _fused_act(self, x: torch.Tensor) -> torch.Tensor | None:
         """The gated hidden activations from jit_thc::gated_linear, or None where it is switched off or does not take them."""
+        if not self.fused_projections:
+            return None
         cast = self.w12.__dict__.get("_cast")
         w, b = cast if cast is not None else (self.w12.weight, self.w12.bias)
         dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
         if not (
-            self.fused_projections
-            and x.is_cuda
+            x.is_cuda
             and dt in (torch.bfloat16, torch.float16)
             and (torch.is_autocast_enabled("cuda") or w.dtype == dt and (b is None or b.dtype == dt))
             and x.shape[-1] % 8 == 0

@@ -309,6 +309,25 @@ def test_gated_linear_stays_off_in_the_model_by_default():
     torch.testing.assert_close(ffn(x), ffn.w3(OB.swiglu_eager(ffn.w12(x))))
 
 
+class Wrapped(torch.nn.Module):
+    """A layer around another, as adapters and loggers are; it has no weight of its own."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x):
+        return self.inner(x) + 1
+
+
+def test_the_feed_forward_runs_a_replaced_projection():
+    from flowmatching_lthc_amd.model import SwiGLUFFN
+
+    ffn, x = SwiGLUFFN(16, 48), torch.randn(3, 16)
+    ffn.w12 = Wrapped(ffn.w12)
+    torch.testing.assert_close(ffn(x), ffn.w3(OB.swiglu_eager(ffn.w12.inner(x) + 1)))
+
+
 def test_adamw_capturable_counts_part_where_steps_part(cpu_kernels):
     """A parameter without a gradient in a step keeps its count, as without capturable."""
     ours, plain = parameters(0), parameters(0)
