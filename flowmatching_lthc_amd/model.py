@@ -342,15 +342,17 @@ class WorkspaceAttention(nn.Module):
 class SwiGLUFFN(nn.Module):
     """SwiGLU MLP with hidden width int(hidden_dim * 2 / 3); w12 output split (gate, value) (local_thc.py:259-269)."""
 
+    # w12, silu and the product as one HIP pass (jit_thc::gated_linear) where it applies.  Off: the eager sequence
+    # rounds the projections to the activation dtype, the fused pass does not.  The class's own, so that modules that were
+    # pickled without it have it too.
+    fused_projections = False
+
     def __init__(self, dim: int, hidden_dim: int, drop: float = 0.0, bias: bool = True) -> None:
         super().__init__()
         hidden = int(hidden_dim * 2 / 3)
         self.w12 = CastLinear(dim, 2 * hidden, bias=bias)
         self.w3 = CastLinear(hidden, dim, bias=bias)
         self.ffn_dropout = nn.Dropout(drop)
-        # w12, silu and the product as one HIP pass (jit_thc::gated_linear) where it applies.  Off: the eager sequence
-        # rounds the projections to the activation dtype, the fused pass does not.
-        self.fused_projections = False
 
     def _fused_act(self, x: torch.Tensor) -> torch.Tensor | None:
         """The gated hidden activations from jit_thc::gated_linear, or None where it is switched off or does not take them."""

@@ -328,6 +328,16 @@ def test_the_feed_forward_runs_a_replaced_projection():
     torch.testing.assert_close(ffn(x), ffn.w3(OB.swiglu_eager(ffn.w12.inner(x) + 1)))
 
 
+def test_a_feed_forward_without_the_switch_in_its_own_state_runs():
+    """As a whole module that was saved before the switch existed."""
+    from flowmatching_lthc_amd.model import SwiGLUFFN
+
+    ffn, x = SwiGLUFFN(16, 48), torch.randn(3, 16)
+    old = SwiGLUFFN.__new__(SwiGLUFFN)
+    old.__dict__.update({k: v for k, v in ffn.__dict__.items() if k != "fused_projections"})
+    assert torch.equal(old(x), ffn(x))
+
+
 def test_adamw_capturable_counts_part_where_steps_part(cpu_kernels):
     """A parameter without a gradient in a step keeps its count, as without capturable."""
     ours, plain = parameters(0), parameters(0)
