@@ -51,6 +51,19 @@ class CastLinear(nn.Linear):
         return y if y is not None else super().forward(x)
 
 
+def _plain_projection(layer: nn.Module) -> bool:
+    """Whether calling `layer` is CastLinear.forward on its weight and bias and nothing else: no other class (a
+    parametrized layer has one of its own), no hooks, no forward set on the instance, no tensor subclass."""
+    return (
+        type(layer) is CastLinear
+        and "forward" not in layer.__dict__
+        and not (layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks or layer._backward_pre_hooks)
+        and not nn.modules.module._has_any_global_hook()
+        and type(layer.weight) in (torch.Tensor, nn.Parameter)
+        and type(layer.bias) in (torch.Tensor, nn.Parameter, type(None))
+    )
+
+
 def _linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """F.linear, its weight and bias gradients from one HIP pass where ops_branch.linear applies."""
     y = ops_branch.linear(x, weight, bias)
@@ -355,15 +368,20 @@ class SwiGLUFFN(nn.Module):
         self.ffn_dropout = nn.Dropout(drop)
 
     def _fused_act(self, x: torch.Tensor) -> torch.Tensor | None:
-        """The gated hidden activations from jit_thc::gated_linear, or None where it is switched off or does not take them."""
-        if not self.fused_projections:
+        """The gated hidden activations from jit_thc::gated_linear, or None where it is switched off, does not take them,
+        or something else than this call would see w12's (a hook, another module in its place, a transform)."""
+        if not (
+            self.fused_projections
+            and x.is_cuda
+            and _plain_projection(self.w12)
+            and (torch.compiler.is_compiling() or type(x) is torch.Tensor and not ops_branch.transformed())
+        ):
             return None
         cast = self.w12.__dict__.get("_cast")
         w, b = cast if cast is not None else (self.w12.weight, self.w12.bias)
         dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
         if not (
-            x.is_cuda
-            and dt in (torch.bfloat16, torch.float16)
+            dt in (torch.bfloat16, torch.float16)
             and (torch.is_autocast_enabled("cuda") or w.dtype == dt and (b is None or b.dtype == dt))
             and x.shape[-1] % 8 == 0
         ):

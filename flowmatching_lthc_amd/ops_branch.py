@@ -336,12 +336,24 @@ def _(grad, x, need_bias):
     return grad.new_empty((n, x.shape[-1])), grad.new_empty((n if need_bias else 0,))
 
 
+def transformed() -> bool:
+    """Whether a TorchScript trace, a functorch or forward-mode transform or a torch function or dispatch mode (a flop
+    counter, for one) sees the calls made here: they know torch's operators."""
+    return (
+        torch.jit.is_tracing()
+        or torch._C._functorch.peek_interpreter_stack() is not None
+        or torch.autograd.forward_ad._current_level >= 0
+        or torch._C._len_torch_dispatch_stack() > 0
+        or any(type(m) is not DeviceContext for m in map(torch._C._get_function_stack_at, range(torch._C._len_torch_function_stack())))
+    )
+
+
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor | None:
     """F.linear(x, weight, bias) with the weight and bias gradients of a training step from linear_weight_grad, or None
     where that does not apply and the caller calls F.linear: no gradient of the weight, not 16-bit products (autocast's,
-    or the operands' own), few rows, a wide weight, or tracing, functorch and forward-mode transforms, tensor subclasses and torch
-    function and dispatch modes (a flop counter, for one), which know torch's linear."""
-    if torch.compiler.is_compiling() or torch.jit.is_tracing() or not (
+    or the operands' own), few rows, a wide weight, or compiling, tensor subclasses and what `transformed` names, which know
+    torch's linear."""
+    if torch.compiler.is_compiling() or not (
         torch.is_grad_enabled()
         and weight.requires_grad
         and type(x) is Tensor
@@ -355,10 +367,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor | None:
         and weight.shape[0] % 8 == 0
         and x.shape[-1] == weight.shape[1]
         and -(-weight.shape[0] // 256) * -(-weight.shape[1] // 128) < LINEAR_MAX_TILES
-        and torch._C._functorch.peek_interpreter_stack() is None
-        and torch.autograd.forward_ad._current_level < 0
-        and torch._C._len_torch_dispatch_stack() == 0
-        and all(type(m) is DeviceContext for m in map(torch._C._get_function_stack_at, range(torch._C._len_torch_function_stack())))
+        and not transformed()
     ):
         return None
     dt = x.dtype

@@ -347,3 +347,30 @@ def test_the_backward_op_computes_what_is_needed(M):
         got = OB.gated_linear_backward(dy, x, w, b, "gelu", *need)
         for n, g, c, t in zip(need, got, full, torch.ops.jit_thc.gated_linear_backward(*(t.to("meta") for t in (dy, x, w, b)), "gelu", *need)):
             assert g.shape == t.shape and (torch.equal(g, c) if n else g.numel() == 0)
+
+
+def test_the_models_feed_forward_calls_a_projection_that_is_more_than_its_weight():
+    """With the switch on too: hooks and other modules in w12's place run, and a function mode sees the call."""
+    from flowmatching_lthc_amd.model import SwiGLUFFN
+
+    print("case gated_linear model with hooks", flush=True)
+    torch.manual_seed(0)
+    ffn = SwiGLUFFN(64, 384).to(DEV, torch.bfloat16)
+    x = randn((2, 50, 64), 0, torch.bfloat16)
+    eager = ffn(x)
+    ffn.fused_projections = True
+    fused = ffn(x)
+    assert not torch.equal(fused, eager)
+    seen = []
+    handle = ffn.w12.register_forward_hook(lambda m, args, out: seen.append(out.shape))
+    assert torch.equal(ffn(x), eager) and len(seen) == 1
+    handle.remove()
+    assert torch.equal(ffn(x), fused)
+    from torch.utils.flop_counter import FlopCounterMode
+
+    with FlopCounterMode(display=False) as flops:
+        assert torch.equal(ffn(x), eager)
+    assert flops.get_total_flops() == 2 * 100 * 64 * 512 + 2 * 100 * 256 * 64
+    inner = ffn.w12
+    ffn.w12 = torch.nn.Sequential(inner, torch.nn.Identity())
+    assert torch.equal(ffn(x), eager)

@@ -7,6 +7,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.testing._internal.two_tensor
 
 from flowmatching_lthc_amd import _abi, optim
 from flowmatching_lthc_amd import ops_branch as OB
@@ -336,6 +337,45 @@ def test_a_feed_forward_without_the_switch_in_its_own_state_runs():
     old = SwiGLUFFN.__new__(SwiGLUFFN)
     old.__dict__.update({k: v for k, v in ffn.__dict__.items() if k != "fused_projections"})
     assert torch.equal(old(x), ffn(x))
+
+
+class Scaled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+def projections():
+    from flowmatching_lthc_amd.model import CastLinear
+
+    class Adapted(CastLinear):
+        def forward(self, x):
+            return super().forward(x) + 1
+
+    def hooked(register):
+        layer = CastLinear(8, 8)
+        getattr(layer, register)(lambda *args: None)
+        return layer
+
+    parametrized, own_forward, subclass = CastLinear(8, 8), CastLinear(8, 8), CastLinear(8, 8)
+    torch.nn.utils.parametrize.register_parametrization(parametrized, "weight", Scaled())
+    own_forward.forward = lambda x: x
+    subclass.weight = torch.nn.Parameter(torch.testing._internal.two_tensor.TwoTensor(torch.ones(8, 8), torch.ones(8, 8)))
+    yield from ((n, hooked("register_" + n)) for n in ("forward_hook", "forward_pre_hook", "full_backward_hook", "full_backward_pre_hook"))
+    yield from (("another module", Wrapped(CastLinear(8, 8))), ("subclass", Adapted(8, 8)), ("parametrized", parametrized))
+    yield from (("forward of its own", own_forward), ("tensor subclass", subclass))
+
+
+def test_the_fused_feed_forward_passes_by_plain_projections_only():
+    from flowmatching_lthc_amd.model import CastLinear, _plain_projection
+
+    assert _plain_projection(CastLinear(8, 8)) and _plain_projection(CastLinear(8, 8, bias=False))
+    for name, layer in projections():
+        assert not _plain_projection(layer), name
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *args: None)
+    try:
+        assert not _plain_projection(CastLinear(8, 8))
+    finally:
+        handle.remove()
 
 
 def test_adamw_capturable_counts_part_where_steps_part(cpu_kernels):
