@@ -7,7 +7,7 @@ of 16-bit parameters and the moving average of the weights that the reference's 
 below it, for programs that hold their states themselves.
 
 Per element, fp32: ``m = m b1 + g (1 - b1)``, ``v = v b2 + g^2 (1 - b2)``,
-``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)``, ``ema = ema d + p (1 - d)``.
+``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)``, ``ema = ema + (p - ema) (1 - d)``.
 
 States in 8 bits: runs of 256 elements share two fp32 scales (A, B) = (max |m|, max v), and the codes c stand for
 ``m = A c |c| / 127^2`` (int8) and ``v = B (c / 255)^4`` (uint8, at least 1 for v > 0).  A value is off by at most half a

@@ -622,7 +622,7 @@ int lthc_axial_rope(const void* q, void* q_out, const int64_t* q_strides, int64_
  * given by host arrays of device pointers; in place, fp32 arithmetic:
  *   g = clip g;  m = m beta1 + g (1 - beta1);  v = v beta2 + g^2 (1 - beta2)
  *   p = p (1 - lr wd) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
- *   ema = ema d + p (1 - d)
+ *   ema = ema + (p - ema) (1 - d)
  * params (p_dtype) and grads (g_dtype) have one dtype each.  masters (NULL:
  * none; 16-bit parameters only): fp32 copies that take the step and are rounded
  * into the parameters.  emas (NULL: none): fp32.  state_bits 32: exp_avgs and

@@ -429,3 +429,27 @@ def test_gradients_may_be_there_twice_but_not_in_written_memory():
         optim.adamw_step([whole[:300]], s.g[:1], s.m[:1], s.v[:1], lr=1e-2, step=whole[:1])
     with pytest.raises(ValueError, match="overlaps"):
         optim.adamw_step([whole[:300]], s.g[:1], s.m[:1], s.v[:1], lr=1e-2, step=1, grad_norm=whole[299:300], max_norm=1.0)
+
+
+@pytest.mark.parametrize("decay", [0.9999, 0.4, 0.0])
+def test_the_moving_average_keeps_no_bias_over_many_steps(decay):
+    """Against the recursion in 64 bits on the same noisy weights, in the mean of 4096 elements.
+
+    A step rounds the difference, its product and the sum: at most U of a value near 1 for the sum, and 1 - d as much of the
+    move for the others.  These roundings fall on either side alike; remembered for 1 / (1 - d) steps they leave
+    0.6 U sqrt(1 / (2 (1 - d))) an element at most, 2.5e-6 at 0.9999, and a 64th of that in the mean: 4e-8.  2e-6 is asked for (3e-5 of an element);
+    weights of d and 1 - d that are rounded by themselves would be off by 1.7e-4 (1 - 0.9999^4000) = 5.5e-5."""
+    print("case adamw moving average", decay, flush=True)
+    n, steps = 4096, 4000 if decay > 0.9 else 50
+    noise = randn((64, n), 1, std=0.05) + 0.8
+    p, g, m, v, e = (torch.zeros(n, device=DEV) for _ in range(5))
+    e.fill_(0.8)
+    want = e.double()
+    for t in range(steps):
+        p.copy_(noise[t % 64].roll(t))
+        optim.adamw_step([p], [g], [m], [v], step=t + 1, lr=0.0, emas=[e], ema_decay=decay)
+        want = want + (p.double() - want) * (1 - decay)
+    assert abs(float((e.double() - want).mean())) <= 2e-6
+    assert float((e.double() - want).abs().max()) <= 3e-5
+    if decay == 0.0:
+        assert torch.equal(e, p)
