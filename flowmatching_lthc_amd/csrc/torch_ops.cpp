@@ -1371,7 +1371,7 @@ LTHC_OP(op_gated_backward, "gated_linear_backward",
         std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
                                            c10::string_view, bool, bool, bool))
 LTHC_OP(replay_gated, "gated_linear_backward_replay",
-        std::vector<Tensor>(const Tensor&, TensorList, c10::string_view, bool))
+        std::vector<Tensor>(const Tensor&, TensorList, c10::string_view))
 LTHC_OP(op_axial_rope, "axial_rope",
         std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, at::IntArrayRef, bool, bool))
 LTHC_OP(op_linear_weight_grad, "linear_weight_grad", std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, bool))
@@ -1922,8 +1922,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
-// The gated linear layer: one backward op for the gradients that are asked for.  Traced, or where a graph of the backward
-// is built, the eager sequence is differentiated.
+// The gated linear layer: one backward op for the gradients that are asked for, traced calls' too: its products are matrix-core
+// work that no compiler makes out of the eager sequence's fp32 ones.  Where a graph of the backward is built, the eager
+// sequence is differentiated.
 struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                         c10::string_view activation) {
@@ -1935,11 +1936,11 @@ struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const auto s = ctx->get_saved_variables();
     const std::string activation = ctx->saved_data["activation"].toStringRef();
-    const bool biased = s[2].defined(), graph = at::GradMode::is_enabled();
-    if (graph || traced(s[0])) {
+    const bool biased = s[2].defined();
+    if (at::GradMode::is_enabled()) {
       std::vector<Tensor> args{s[0], s[1]};
       if (biased) args.push_back(s[2]);
-      return wanted(ctx, replay_gated().call(grads[0], args, activation, graph), 4);
+      return wanted(ctx, replay_gated().call(grads[0], args, activation), 4);
     }
     DetachedScope scope;
     const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), biased && ctx->needs_input_grad(2)};

@@ -37,7 +37,8 @@ op's inputs and gives the gradients of the eager sequence.  For batched
 gradients (is_grads_batched, vmap) torch runs that pass once per sample.  A
 traced backward (torch.compile) differentiates the eager sequence in place of
 those kernels (gate_residual's apart, which rounds nothing in between): the
-compiled graph keeps the chain's intermediates in fp32.
+compiled graph keeps the chain's intermediates in fp32.  The gated linear
+layer's backward, which is matrix products, is its op in a traced graph too.
 """
 
 from __future__ import annotations
@@ -402,8 +403,8 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activati
     none, activation silu, gelu or gelu_tanh: the w12 projection and gate of SwiGLUFFN in one matrix-core pass, the
     projections in fp32 up to the one rounding of the result.
 
-    bf16 or fp16 (under autocast, its dtype), C a multiple of 8, any F.  The backward recomputes the projections; a second
-    derivative goes through gated_linear_eager."""
+    bf16 or fp16 (under autocast, its dtype), C a multiple of 8, any F.  The backward, a compiled one too, is
+    gated_linear_backward, which recomputes the projections; a second derivative goes through gated_linear_eager."""
     _refuse(x)
 
 
@@ -428,17 +429,15 @@ def _(grad, x, weight, bias, activation, need_x, need_weight, need_bias):
     return gx, x.new_empty((n if need_weight else 0, weight.shape[1])), x.new_empty((n if need_bias else 0,))
 
 
-def _gated_linear_replay(grad: Tensor, args: list[Tensor], activation: str, graph: bool) -> list[Tensor]:
+def _gated_linear_replay(grad: Tensor, args: list[Tensor], activation: str) -> list[Tensor]:
     with torch.enable_grad():
-        if not graph:
-            args = [t.detach().requires_grad_() for t in args]
-        else:  # leaves that ask for no gradient take part in the differentiation all the same
-            args = [t if t.requires_grad else t.detach().requires_grad_() for t in args]
+        # leaves that ask for no gradient take part in the differentiation all the same
+        args = [t if t.requires_grad else t.detach().requires_grad_() for t in args]
         out = gated_linear_eager(args[0], args[1], args[2] if len(args) > 2 else None, activation)
-        return list(torch.autograd.grad(out, args, grad, create_graph=graph))
+        return list(torch.autograd.grad(out, args, grad, create_graph=True))
 
 
-torch.library.define("jit_thc::gated_linear_backward_replay", "(Tensor grad, Tensor[] args, str activation, bool graph) -> Tensor[]")
+torch.library.define("jit_thc::gated_linear_backward_replay", "(Tensor grad, Tensor[] args, str activation) -> Tensor[]")
 torch.library.impl("jit_thc::gated_linear_backward_replay", "CompositeImplicitAutograd")(_gated_linear_replay)
 
 

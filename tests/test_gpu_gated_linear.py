@@ -374,3 +374,39 @@ def test_the_models_feed_forward_calls_a_projection_that_is_more_than_its_weight
     inner = ffn.w12
     ffn.w12 = torch.nn.Sequential(inner, torch.nn.Identity())
     assert torch.equal(ffn(x), eager)
+
+
+def test_the_models_feed_forward_compiles_to_the_kernels():
+    """The compiled forward and backward of SwiGLUFFN with the switch on hold the two operators and the products of w3 alone,
+    none of them in fp32, and give the eager call's values."""
+    from functorch.compile import make_boxed_func
+    from torch._dynamo.backends.common import aot_autograd
+
+    from flowmatching_lthc_amd.model import SwiGLUFFN
+
+    print("case gated_linear compiled model", flush=True)
+    torch._dynamo.reset()
+    torch.manual_seed(0)
+    ffn = SwiGLUFFN(64, 384).to(DEV, torch.bfloat16)
+    ffn.fused_projections = True
+    x = randn((2, 50, 64), 0, torch.bfloat16).requires_grad_()
+    dy = randn((2, 50, 64), 1, torch.bfloat16)
+    graphs = []
+
+    def keep(graph, inputs):
+        graphs.append([n for n in graph.graph.nodes if n.op == "call_function"])
+        return make_boxed_func(graph.forward)
+
+    y = torch.compile(ffn, backend=aot_autograd(fw_compiler=keep, bw_compiler=keep), fullgraph=True)(x)
+    got = [y, *torch.autograd.grad(y, [x, *ffn.parameters()], dy)]
+    assert len(graphs) == 2
+    for nodes, op in zip(graphs, ("gated_linear", "gated_linear_backward")):
+        assert f"jit_thc.{op}.default" in {str(n.target) for n in nodes}
+        products = [n for n in nodes if any(p in str(n.target) for p in ("aten.mm", "aten.addmm", "aten.bmm"))]
+        assert len(products) == (1 if op == "gated_linear" else 2)
+        assert all(n.meta["val"].dtype == torch.bfloat16 for n in products)
+    want = ffn(x)
+    for a, c in zip(got, [want, *torch.autograd.grad(want, [x, *ffn.parameters()], dy)]):
+        # w3's own products may be split differently: a rounding of their results
+        assert float((a - c).detach().abs().max()) <= 2**-7 * float(c.detach().abs().max())
+    torch._dynamo.reset()
