@@ -577,8 +577,7 @@ int lthc_interface_bwd(const void* gx, const void* const* gz, int x_dtype, const
  * multiple of 8; any F and M; x and weight 16-byte aligned, 4 F C < 2^31 - 2^24.
  * Backward for dy [M, F]: dx [M, C], dw [2F, C] and db [2F], each NULL where it is
  * not wanted.  The projections are recomputed; their gradients
- * are rounded to x_dtype once, where they enter the products of dx and dw, and in
- * small calls (M 2F <= 65536) enter them as two values, the rounded one and the rest.
+ * are rounded to x_dtype once, where they enter the products of dx and dw.
  */
 #define LTHC_ACT_SILU 0
 #define LTHC_ACT_GELU 1

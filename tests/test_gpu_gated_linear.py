@@ -410,3 +410,18 @@ def test_the_models_feed_forward_compiles_to_the_kernels():
         # w3's own products may be split differently: a rounding of their results
         assert float((a - c).detach().abs().max()) <= 2**-7 * float(c.detach().abs().max())
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(64, 512, (1, 32, 64, 65, 700)), (64, 24, (5, 1365, 1366, 53000)), (1024, 1024, (3, 32, 33))], ids=str)
+def test_a_rows_gradient_does_not_depend_on_the_rows_beside_it(shape, dtype):
+    """dx of the first rows of a batch is that of the rows by themselves, bit for bit: sums in the same order and the same
+    roundings at every number of rows."""
+    C, F, rows = shape
+    print("case gated_linear rows alone", shape, dtype, flush=True)
+    x, w, b = operands(rows[-1], C, F, dtype)
+    dy = randn((rows[-1], F), 9, dtype)
+    whole, _, _ = OB.gated_linear_backward(dy, x, w, b, "silu", True, False, False)
+    for M in rows[:-1]:
+        dx, _, _ = OB.gated_linear_backward(dy[:M], x[:M], w, b, "silu", True, False, False)
+        assert torch.equal(dx, whole[:M]), M
