@@ -167,6 +167,10 @@ class AdamW(torch.optim.Optimizer):
         )  # fmt: skip
         super().__init__(params, defaults)
 
+    def __getstate__(self) -> dict:
+        """What copies and pickles hold: torch's optimizers give theirs by name."""
+        return {**super().__getstate__(), "max_norm": self.max_norm, "last_grad_norm": self.last_grad_norm}
+
     # ------------------------------------------------------------------ state
     def _init_state(self, p: Tensor, group: dict) -> dict:
         state = self.state[p]

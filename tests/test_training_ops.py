@@ -415,3 +415,20 @@ def test_gated_linear_workspace_of_sizes_out_of_range():
     for sizes in ((0, 8, 8), (8, -8, 8), (1 << 40, 8, 8), (8, 1 << 40, 8), (8, 8, 1 << 40), (8, 1 << 19, 1 << 19), (-1, 1 << 62, 1 << 62)):
         assert query(*sizes) == 0, sizes
     assert query(8, 8, 8) > 0
+
+
+def test_adamw_copies_and_pickles(cpu_kernels, tmp_path):
+    params = parameters(0)
+    a = optim.AdamW(params, lr=1e-2, max_norm=0.5, ema_decay=0.9)
+    run(a, params, 2)
+    held = [a.state[p]["exp_avg"] for p in params]
+    torch.save(a, tmp_path / "opt.pt")
+    copies = [copy.deepcopy(a), torch.load(tmp_path / "opt.pt", weights_only=False)]
+    run(a, params, 1, seed=7)
+    for b in copies:
+        others = b.param_groups[0]["params"]
+        assert b.max_norm == 0.5 and b.last_grad_norm is not None
+        run(b, others, 1, seed=7)
+        for p, q in zip(params, others):
+            assert p is not q and torch.equal(p, q) and torch.equal(a.state[p]["ema"], b.state[q]["ema"])
+    assert all(a.state[p]["exp_avg"] is h for p, h in zip(params, held))
