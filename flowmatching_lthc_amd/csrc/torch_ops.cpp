@@ -2090,7 +2090,15 @@ Tensor gres_autograd(const Tensor& d, const Tensor& gate, const Tensor& m) {
   return op_gres().call(d, gate, m);
 }
 
+// These kernels compute no tangents: a call with one would lose it.
+void no_tangents(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+
 Tensor gated_autograd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, c10::string_view activation) {
+  const Tensor none;
+  no_tangents("gated_linear", {&x, &weight, given(bias) ? &*bias : &none});
   if (recording(x, weight) || (given(bias) && recording(*bias))) return GatedLinearFn::apply(x, weight, bias, activation);
   BelowAutograd below;
   return op_gated().call(x, weight, bias, activation);
@@ -2107,6 +2115,7 @@ Tensor gated_autocast(const Tensor& x, const Tensor& weight, const std::optional
 std::tuple<Tensor, Tensor> axial_rope_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
                                                at::IntArrayRef sections, bool interleaved, bool inverse) {
   TORCH_CHECK_VALUE(!recording(positions, inv_freq), "axial_rope gives no gradient of positions or inv_freq");
+  no_tangents("axial_rope", {&q, &k, &positions, &inv_freq});
   if (recording(q, k)) return pair(AxialRopeFn::apply(q, k, positions, inv_freq, sections, interleaved, inverse));
   BelowAutograd below;
   return op_axial_rope().call(q, k, positions, inv_freq, sections, interleaved, inverse);

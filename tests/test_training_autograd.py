@@ -84,3 +84,22 @@ def test_batched_gradients_are_those_of_each_sample(node):
         vmapped = torch.vmap(lambda *g: torch.autograd.grad(outs, leaves[want], g, retain_graph=True))(*grads)
         for a, v, b in zip(got, vmapped, zip(*(e[want] for e in each))):
             assert torch.equal(a, torch.stack(b)) and torch.equal(v, a)
+
+
+@pytest.mark.parametrize("recorded", [True, False])
+@pytest.mark.parametrize("node", [gated, rope])
+def test_forward_mode_is_refused(node, recorded):
+    """A tangent is not lost without a word."""
+
+    def call(*args):
+        return OB.gated_linear(*args) if node is gated else OB.axial_rope(*args, torch.zeros(3, 1), torch.ones(4).double(), (8,))
+
+    leaves, _ = node()
+    for i in range(len(leaves)):
+        args = [t.detach().requires_grad_(recorded) for t in leaves]
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*args[:i], dual, *args[i + 1 :])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: call(*args[:i], t, *args[i + 1 :]), (args[i].detach(),), (args[i].detach(),))
