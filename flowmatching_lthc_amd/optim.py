@@ -174,9 +174,12 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def _init_state(self, p: Tensor, group: dict) -> dict:
         state = self.state[p]
-        missing = "exp_avg" not in state or (
-            group["master_weights"] and p.dtype != torch.float32 and "master" not in state
-        ) or (group["ema_decay"] is not None and "ema" not in state)  # fmt: skip
+        missing = (
+            "exp_avg" not in state
+            or (group["master_weights"] and p.dtype != torch.float32 and "master" not in state)
+            or (group["ema_decay"] is not None and "ema" not in state)
+            or (group["capturable"] and not isinstance(state["step"], Tensor))
+        )
         if missing and _capturing(p):
             raise RuntimeError("a captured AdamW step needs its states: take one step outside the capture first")
         if "exp_avg" not in state:

@@ -432,3 +432,22 @@ def test_adamw_copies_and_pickles(cpu_kernels, tmp_path):
         for p, q in zip(params, others):
             assert p is not q and torch.equal(p, q) and torch.equal(a.state[p]["ema"], b.state[q]["ema"])
     assert all(a.state[p]["exp_avg"] is h for p, h in zip(params, held))
+
+
+def test_a_capture_right_after_capturable_is_set_is_refused(cpu_kernels, monkeypatch):
+    """Counts that are still the host's would be captured as constants: every replay would take the same step."""
+    first, params = parameters(0), parameters(0)
+    a = optim.AdamW(first, lr=1e-2)
+    run(a, first, 2)
+    b = optim.AdamW(params, lr=1e-2, capturable=True)
+    b.load_state_dict(a.state_dict())  # a saved group's options are the optimizer's: not capturable
+    b.param_groups[0]["capturable"] = True
+    capturing = True
+    monkeypatch.setattr(optim, "_capturing", lambda t: capturing)
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        run(b, params, 1)
+    capturing = False
+    run(b, params, 1)
+    capturing = True
+    run(b, params, 1)
+    assert all(float(b.state[p]["step"]) == 4 for p in params)
