@@ -451,3 +451,35 @@ def test_a_capture_right_after_capturable_is_set_is_refused(cpu_kernels, monkeyp
     capturing = True
     run(b, params, 1)
     assert all(float(b.state[p]["step"]) == 4 for p in params)
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_adamw_groups_take_their_own_options(cpu_kernels, capturable):
+    """Two groups of unlike types and options, one norm over both, against torch's optimizer on clipped gradients; a third
+    group added later counts its own steps."""
+    small = parameters(0), parameters(1, torch.bfloat16), parameters(2)
+    ours, theirs = ([[torch.nn.Parameter(p.detach().clone()) for p in ps] for ps in small] for _ in range(2))
+    options = (dict(lr=1e-2, weight_decay=0.1, ema_decay=0.5), dict(lr=3e-2, betas=(0.5, 0.8)), dict(lr=1e-3, eps=1e-4))
+    plain = [{k: v for k, v in o.items() if k != "ema_decay"} for o in options]
+    a = optim.AdamW([{"params": ps, **o} for ps, o in zip(ours[:2], options)], max_norm=0.5, capturable=capturable)
+    b = torch.optim.AdamW([{"params": ps, **o} for ps, o in zip(theirs[:2], plain)])
+    for t in range(5):
+        if t == 3:
+            a.add_param_group({"params": ours[2], **options[2]})
+            b.add_param_group({"params": theirs[2], **plain[2]})
+        gen = torch.Generator().manual_seed(50 + t)
+        grads = [[torch.randn(p.shape, generator=gen).to(p.dtype) for p in ps] for ps in small[: len(a.param_groups)]]
+        clip = 0.5 / (torch.linalg.vector_norm(torch.cat([g.flatten().float() for gs in grads for g in gs])) + 1e-6)
+        for mine, other, gs in zip(ours, theirs, grads):
+            for p, q, g in zip(mine, other, gs):
+                p.grad, q.grad = g, (g.float() * clip).to(g.dtype)
+        a.step()
+        b.step()
+    for mine, other in zip(ours, theirs):
+        for p, q in zip(mine, other):
+            # bf16: five steps' weights are rounded (2^-8 each), and there the states and the clipped gradients too, whose
+            # steps of 3e-2 they move by a few 2^-8 more
+            rtol, atol = (1e-5, 1e-6) if p.dtype == torch.float32 else (6 * 2.0**-8, 5 * 3e-2 * 8 * 2.0**-8)
+            torch.testing.assert_close(p, q, rtol=rtol, atol=atol)
+            assert float(a.state[p]["step"]) == float(b.state[q]["step"])
+    assert all("ema" in a.state[p] for p in ours[0]) and not any("ema" in a.state[p] for p in (*ours[1], *ours[2]))
