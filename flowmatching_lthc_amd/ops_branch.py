@@ -404,7 +404,9 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activati
     projections in fp32 up to the one rounding of the result.
 
     bf16 or fp16 (under autocast, its dtype), C a multiple of 8, any F.  The backward, a compiled one too, is
-    gated_linear_backward, which recomputes the projections; a second derivative goes through gated_linear_eager."""
+    gated_linear_backward, which recomputes the projections; a second derivative goes through gated_linear_eager.  The
+    projections' gradients are rounded to x's dtype once, where they enter the products of the others: fp16 ones need a loss
+    scale that keeps them within its range (6e-5 to 65504).  No forward-mode derivative."""
     _refuse(x)
 
 
@@ -457,7 +459,8 @@ def axial_rope(
     axes) and turns by the angle positions[..., a] * inv_freq[p], a product in 64 bits; the channels past R are copied.
     positions [N, A] (one map for the batch) or [B, N, A], int32, int64, float32 or float64; inv_freq float64 [R / 2].
     inverse: by the negative angle, which is the gradient's rotation.  Heads with 0 entries are left out.  Outputs have
-    their inputs' layout where that is dense, and are contiguous otherwise.  No gradient of positions or inv_freq."""
+    their inputs' layout where that is dense, and are contiguous otherwise.  No gradient of positions or inv_freq, no
+    forward-mode derivative."""
     _refuse(q)
 
 

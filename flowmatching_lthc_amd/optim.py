@@ -80,7 +80,8 @@ def adamw_step(
 
     params and grads have one dtype each, of fp32, bf16 and fp16.  exp_avgs and exp_avg_sqs are fp32 in their parameters'
     layout, or, with `scales` (fp32 [2, runs of 256]), contiguous int8 and uint8 codes.  masters: fp32 copies of 16-bit
-    parameters, which take the step and are rounded into them.  emas: fp32 moving averages.  grad_norm: the norm of all
+    parameters, which take the step and are rounded into them.  emas: fp32 moving averages of the step's fp32 result (of a
+    16-bit parameter without a master too, before it is rounded).  grad_norm: the norm of all
     gradients (one fp32 on the device); they are scaled by min(1, max_norm / (grad_norm + 1e-6)), and where it is not finite
     nothing is changed.  What the step writes lies in memory of its own; a gradient may be there twice.  step and lr may be
     one fp32 on the device, which a captured graph reads anew on each replay."""
@@ -120,7 +121,9 @@ class AdamW(torch.optim.Optimizer):
       ones, whose state costs nothing, keep 32 bits;
     * ``master_weights``: fp32 copies of 16-bit parameters, which take the steps (``state[p]["master"]``);
     * ``ema_decay``: fp32 moving averages of the weights (``state[p]["ema"]``, ``ema_params``), begun at the weights of a
-      parameter's first step;
+      parameter's first step.  An average takes the step's fp32 result, and moves in its parameter's steps only: a parameter
+      without a gradient, or a step that is left out for its norm, leaves it as it is (an update of its own after every
+      step, as in the reference's training script, would go on towards the weights there);
     * ``max_norm``: clipping by the norm of all gradients, which ``last_grad_norm`` keeps on the device; a step whose norm is
       not finite changes no tensor (it is counted);
     * ``capturable``: step counts on the device, one for all parameters that have taken the same steps, and a learning rate

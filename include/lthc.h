@@ -576,8 +576,10 @@ int lthc_interface_bwd(const void* gx, const void* const* gz, int x_dtype, const
  * in fp32, rounded once.  act: LTHC_ACT_SILU, _GELU (erf), _GELU_TANH.  C a
  * multiple of 8; any F and M; x and weight 16-byte aligned, 4 F C < 2^31 - 2^24.
  * Backward for dy [M, F]: dx [M, C], dw [2F, C] and db [2F], each NULL where it is
- * not wanted.  The projections are recomputed; their gradients
- * are rounded to x_dtype once, where they enter the products of dx and dw.
+ * not wanted.  The projections are recomputed; their gradients are rounded to x_dtype
+ * once, where they enter the products of dx and dw.  In fp16, as in an eager fp16
+ * backward, they overflow past 65504 and lose digits below 6e-5, also where dx and dw
+ * would not: scale the loss so that they lie in between.
  */
 #define LTHC_ACT_SILU 0
 #define LTHC_ACT_GELU 1
@@ -624,9 +626,11 @@ int lthc_axial_rope(const void* q, void* q_out, const int64_t* q_strides, int64_
  *   ema = ema + (p - ema) (1 - d)
  * params (p_dtype) and grads (g_dtype) have one dtype each.  masters (NULL:
  * none; 16-bit parameters only): fp32 copies that take the step and are rounded
- * into the parameters.  emas (NULL: none): fp32.  state_bits 32: exp_avgs and
- * exp_avg_sqs are fp32.  8: they are int8 and uint8 codes of runs of 256
- * elements (the last one may be shorter), scales[i] fp32 [2, runs] = (A, B):
+ * into the parameters.  emas (NULL: none): fp32, of the step's fp32 result p
+ * (before it is rounded into a 16-bit parameter, with a master or without).
+ * state_bits 32: exp_avgs and exp_avg_sqs are fp32.  8: they are int8 and uint8
+ * codes of runs of 256 elements (the last one may be shorter), scales[i] fp32
+ * [2, runs] = (A, B):
  *   m = A c |c| / 127^2,  v = B (c / 255)^4
  * grad_norm (NULL: no clipping): the norm of all gradients on the device; clip =
  * min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves every
