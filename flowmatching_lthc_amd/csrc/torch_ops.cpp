@@ -1922,9 +1922,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
-// The gated linear layer: one backward op for the gradients that are asked for, traced calls' too: its products are matrix-core
-// work that no compiler makes out of the eager sequence's fp32 ones.  Where a graph of the backward is built, the eager
-// sequence is differentiated.
+// The gated linear layer: one backward op for the gradients that are asked for, traced calls' too: a compiler would make
+// fp32 products of the eager sequence.  Where a graph of the backward is built, that sequence is differentiated.
 struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                         c10::string_view activation) {
