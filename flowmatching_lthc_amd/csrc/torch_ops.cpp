@@ -1107,6 +1107,209 @@ std::tuple<Tensor, Tensor> axial_rope_cuda(const Tensor& q_, const Tensor& k_, c
 }
 
 // ---------------------------------------------------------------------------
+// inference in 8-bit integers
+// ---------------------------------------------------------------------------
+int64_t up16(int64_t c) { return (c + 15) / 16 * 16; }
+
+// [..., C] as rows that lie one distance apart: a view where the strides allow it, else a copy.
+struct Rows {
+  Tensor t;
+  int64_t ld;
+  explicit Rows(const Tensor& x) : t(x) {
+    const int64_t d = t.dim(), c = t.size(d - 1);
+    bool even = t.stride(d - 1) == 1 || c == 1;
+    int64_t step = 0, count = 1;  // of the rows so far
+    for (int64_t i = d - 2; i >= 0 && even; --i) {
+      if (t.size(i) == 1) continue;
+      if (count == 1) step = t.stride(i);
+      else even = t.stride(i) == step * count;
+      count *= t.size(i);
+    }
+    ld = count == 1 ? c : step;
+    if (even) return;
+    t = t.contiguous();
+    ld = c;
+  }
+};
+
+// The same for int8 rows, which the products load in aligned pieces of 16.
+struct Int8Rows : Rows {
+  explicit Int8Rows(const Tensor& x) : Rows(x) {
+    if (ld % 16 == 0 && aligned(t, 16)) return;
+    t = t.clone(at::MemoryFormat::Contiguous);
+    ld = t.size(-1);
+  }
+};
+
+void check_channels(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, name, " [..., C] with at least one channel expected, got ", shape(x));
+}
+
+std::tuple<Tensor, Tensor> empty_rows(const Tensor& x) {  // (q [..., up16(C)], scales [...])
+  auto sizes = x.sizes().vec();
+  sizes.back() = up16(sizes.back());
+  return {at::empty(sizes, x.options().dtype(at::kChar)), fp32_like(x.sizes().slice(0, x.dim() - 1), x)};
+}
+
+std::tuple<Tensor, Tensor> quantize_rows_cuda(const Tensor& x_) {
+  on_gpu(x_);
+  check_channels(x_, "x");
+  const int dt = code(x_);
+  const Rows x(x_);
+  auto [q, s] = empty_rows(x_);
+  const Launch l(x_);
+  check(lthc_quantize_rows(data(x.t), dt, x.ld, q.data_ptr<int8_t>(), s.data_ptr<float>(), s.numel(), x_.size(-1), l.stream),
+        "lthc_quantize_rows");
+  return {q, s};
+}
+
+void check_scales(const Tensor& q, const Tensor& s, const char* name) {
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.dim() >= 1 && q.size(-1) > 0 && q.size(-1) % 16 == 0, name,
+                    " must be int8 rows [..., K] with K a multiple of 16, got ", shape(q), " ", q.scalar_type());
+  TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.sizes() == q.sizes().slice(0, q.dim() - 1), name,
+                    "'s scales must be float32, one for each row, got ", shape(s), " ", s.scalar_type(), " for ", shape(q));
+  on_gpu(q, s);
+}
+
+Tensor dequantize_rows_cuda(const Tensor& q_, const Tensor& scale, int64_t channels, at::ScalarType dtype) {
+  check_scales(q_, scale, "q");
+  TORCH_CHECK_VALUE(channels > 0 && channels <= q_.size(-1), "channels must be 1 to ", q_.size(-1), ", got ", channels);
+  const Int8Rows q(q_);
+  const Tensor s = scale.contiguous();
+  auto sizes = q_.sizes().vec();
+  sizes.back() = channels;
+  Tensor out = at::empty(sizes, q_.options().dtype(dtype));
+  const int dt = code(out);
+  const Launch l(q_);
+  // rows that are one and the same have to be told apart by a row's length at least
+  const Tensor t = q.ld < q_.size(-1) ? q.t.contiguous() : q.t;
+  check(lthc_dequantize_rows(t.data_ptr<int8_t>(), q.ld < q_.size(-1) ? q_.size(-1) : q.ld, s.data_ptr<float>(), data(out), dt, s.numel(),
+                             channels, l.stream),
+        "lthc_dequantize_rows");
+  return out;
+}
+
+// A row [C] for all samples or [B, C], its channels consecutive: (tensor, elements between samples).
+std::pair<Tensor, int64_t> sample_rows(const Tensor& t_, const Tensor& x, const char* name) {
+  const int64_t c = x.size(-1);
+  TORCH_CHECK_VALUE((t_.dim() == 1 && t_.size(0) == c) || (x.dim() == 3 && has_shape(t_, {x.size(0), c})), name, " must be [", c,
+                    "], or [B,", c, "] for x [B,N,", c, "], got ", shape(t_), " for ", shape(x));
+  code(t_);
+  same_device(x, t_);
+  const Tensor t = t_.stride(-1) == 1 || c == 1 ? t_ : t_.contiguous();
+  return {t, t.dim() == 1 ? 0 : t.stride(0)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_quantize_cuda(const Tensor& x_, const Tensor& weight, double eps,
+                                                      const std::optional<Tensor>& residual_, const std::optional<Tensor>& gate_,
+                                                      const std::optional<Tensor>& shift_, const std::optional<Tensor>& scale_,
+                                                      c10::string_view keep) {
+  on_gpu(x_, weight);
+  check_channels(x_, "x");
+  const int dt = code(x_);
+  const int64_t c = x_.size(-1);
+  TORCH_CHECK_VALUE(has_shape(weight, {c}), "weight must be [", c, "], got ", shape(weight));
+  TORCH_CHECK_VALUE(keep == "none" || keep == "sum" || keep == "update", "keep must be none, sum or update, got ", keep);
+  TORCH_CHECK_VALUE(given(shift_) == given(scale_), "shift and scale come together");
+  const int kept = keep == "sum" ? LTHC_KEEP_SUM : keep == "update" ? LTHC_KEEP_UPDATE : LTHC_KEEP_NONE;
+  const Rows x(x_);
+  Rows residual = x;
+  if (given(residual_)) {
+    TORCH_CHECK_VALUE(residual_->sizes() == x_.sizes() && residual_->scalar_type() == x_.scalar_type(),
+                      "residual must have x's shape and dtype ", shape(x_), " ", x_.scalar_type(), ", got ", shape(*residual_), " ",
+                      residual_->scalar_type());
+    same_device(x_, *residual_);
+    residual = Rows(*residual_);
+  }
+  std::pair<Tensor, int64_t> gate{}, shift{}, scale{};
+  if (given(gate_)) gate = sample_rows(*gate_, x_, "gate");
+  if (given(shift_)) {
+    shift = sample_rows(*shift_, x_, "shift");
+    scale = sample_rows(*scale_, x_, "scale");
+    TORCH_CHECK_VALUE(shift.first.sizes() == scale.first.sizes() && shift.first.scalar_type() == scale.first.scalar_type(),
+                      "shift and scale must have one shape and dtype");
+    if (shift.second != scale.second) {
+      shift = {shift.first.contiguous(), c};
+      scale = {scale.first.contiguous(), c};
+    }
+  }
+  const Tensor w = (known_dtype(weight) ? weight : weight.to(at::kFloat)).contiguous();
+  auto [q, s] = empty_rows(x_);
+  Tensor out = kept == LTHC_KEEP_NONE ? at::empty({0}, x_.options()) : at::empty(x_.sizes(), x_.options());
+  // [B, N, C]: N rows a sample; otherwise one sample
+  const int64_t n = x_.dim() == 3 ? x_.size(1) : s.numel(), b = x_.dim() == 3 ? x_.size(0) : 1;
+  const auto at = [](const Tensor& t) { return t.defined() ? data(t) : nullptr; };
+  const auto type = [](const Tensor& t) { return t.defined() ? code(t) : LTHC_F32; };
+  const Launch l(x_);
+  check(lthc_norm_quantize(data(x.t), dt, x.ld, given(residual_) ? data(residual.t) : nullptr, residual.ld, at(gate.first),
+                           type(gate.first), gate.second, data(w), code(w), at(shift.first), at(scale.first), type(shift.first),
+                           shift.second, kept, kept ? data(out) : nullptr, q.data_ptr<int8_t>(), s.data_ptr<float>(), b, n, c,
+                           static_cast<float>(eps), l.stream),
+        "lthc_norm_quantize");
+  return {out, q, s};
+}
+
+struct Int8Operands {
+  Int8Rows q, w;
+  Tensor s, v, b;
+  std::vector<int64_t> sizes;  // of the result but for its last one
+  Int8Operands(const Tensor& q_, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias)
+      : q(checked(q_, scale, weight, weight_scale, bias)), w(weight), s(scale.contiguous()), v(weight_scale.contiguous()) {
+    if (w.ld < weight.size(1)) {  // a weight of one row that is repeated
+      w.t = w.t.contiguous();
+      w.ld = weight.size(1);
+    }
+    if (given(bias)) b = bias->to(at::kFloat).contiguous();
+    sizes = q_.sizes().vec();
+  }
+  static const Tensor& checked(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                               const std::optional<Tensor>& bias) {
+    check_scales(q, scale, "q");
+    TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) > 0, "weight must be [N, K], got ", shape(weight));
+    check_scales(weight, weight_scale, "weight");
+    TORCH_CHECK_VALUE(weight.size(1) == q.size(-1), "q [..., K] and weight [N, K] expected, got ", shape(q), " and ", shape(weight));
+    on_gpu(q, weight);
+    if (given(bias)) {
+      TORCH_CHECK_VALUE(has_shape(*bias, {weight.size(0)}), "bias must be [", weight.size(0), "], got ", shape(*bias));
+      code(*bias);
+      on_gpu(q, *bias);
+    }
+    return q;
+  }
+  const float* bias() const { return b.defined() ? b.data_ptr<float>() : nullptr; }
+};
+
+Tensor int8_linear_cuda(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                        const std::optional<Tensor>& bias, at::ScalarType dtype) {
+  const Int8Operands o(q, scale, weight, weight_scale, bias);
+  auto sizes = o.sizes;
+  sizes.back() = weight.size(0);
+  Tensor y = at::empty(sizes, q.options().dtype(dtype));
+  const int dt = code(y);
+  const Launch l(q);
+  check(lthc_int8_linear(o.q.t.data_ptr<int8_t>(), o.q.ld, o.s.data_ptr<float>(), o.w.t.data_ptr<int8_t>(), o.w.ld, o.v.data_ptr<float>(),
+                         o.bias(), data(y), dt, o.s.numel(), weight.size(0), weight.size(1), l.stream),
+        "lthc_int8_linear");
+  return y;
+}
+
+Tensor int8_gated_linear_cuda(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                              const std::optional<Tensor>& bias, c10::string_view activation, at::ScalarType dtype) {
+  const int act = act_code(activation);
+  const Int8Operands o(q, scale, weight, weight_scale, bias);
+  TORCH_CHECK_VALUE(weight.size(0) % 2 == 0, "weight must be [2F, K], got ", shape(weight));
+  auto sizes = o.sizes;
+  sizes.back() = weight.size(0) / 2;
+  Tensor y = at::empty(sizes, q.options().dtype(dtype));
+  const int dt = code(y);
+  const Launch l(q);
+  check(lthc_int8_gated_linear(o.q.t.data_ptr<int8_t>(), o.q.ld, o.s.data_ptr<float>(), o.w.t.data_ptr<int8_t>(), o.w.ld,
+                               o.v.data_ptr<float>(), o.bias(), act, data(y), dt, o.s.numel(), sizes.back(), weight.size(1), l.stream),
+        "lthc_int8_gated_linear");
+  return y;
+}
+
+// ---------------------------------------------------------------------------
 // AdamW over many tensors
 // ---------------------------------------------------------------------------
 constexpr int64_t kAdamRun = 256;  // elements that share a scale of an 8-bit state
@@ -1374,6 +1577,17 @@ LTHC_OP(replay_gated, "gated_linear_backward_replay",
         std::vector<Tensor>(const Tensor&, TensorList, c10::string_view))
 LTHC_OP(op_axial_rope, "axial_rope",
         std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, at::IntArrayRef, bool, bool))
+LTHC_OP(op_quantize_rows, "quantize_rows", std::tuple<Tensor, Tensor>(const Tensor&))
+LTHC_OP(op_dequantize_rows, "dequantize_rows", Tensor(const Tensor&, const Tensor&, c10::SymInt, at::ScalarType))
+LTHC_OP(op_norm_quantize, "norm_quantize",
+        std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, double, const std::optional<Tensor>&,
+                                           const std::optional<Tensor>&, const std::optional<Tensor>&,
+                                           const std::optional<Tensor>&, c10::string_view))
+LTHC_OP(op_int8_linear, "int8_linear",
+        Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, at::ScalarType))
+LTHC_OP(op_int8_gated_linear, "int8_gated_linear",
+        Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, c10::string_view,
+               at::ScalarType))
 LTHC_OP(op_linear_weight_grad, "linear_weight_grad", std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, bool))
 
 using BelowAutograd = at::AutoDispatchBelowADInplaceOrView;
@@ -2120,6 +2334,55 @@ std::tuple<Tensor, Tensor> axial_rope_autograd(const Tensor& q, const Tensor& k,
   return op_axial_rope().call(q, k, positions, inv_freq, sections, interleaved, inverse);
 }
 
+// 8-bit operators: rounding has no gradient, and a call that autograd records would lose it.
+void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_VALUE(!recording(*t), op, " has no gradient: call it under torch.no_grad()");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+  }
+}
+
+const Tensor& or_none(const std::optional<Tensor>& t) {
+  static const Tensor none;
+  return given(t) ? *t : none;
+}
+
+std::tuple<Tensor, Tensor> quantize_rows_autograd(const Tensor& x) {
+  no_gradient("quantize_rows", {&x});
+  BelowAutograd below;
+  return op_quantize_rows().call(x);
+}
+
+Tensor dequantize_rows_autograd(const Tensor& q, const Tensor& scale, c10::SymInt channels, at::ScalarType dtype) {
+  no_gradient("dequantize_rows", {&scale});
+  BelowAutograd below;
+  return op_dequantize_rows().call(q, scale, channels, dtype);
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_quantize_autograd(const Tensor& x, const Tensor& weight, double eps,
+                                                          const std::optional<Tensor>& residual, const std::optional<Tensor>& gate,
+                                                          const std::optional<Tensor>& shift, const std::optional<Tensor>& scale,
+                                                          c10::string_view keep) {
+  no_gradient("norm_quantize", {&x, &weight, &or_none(residual), &or_none(gate), &or_none(shift), &or_none(scale)});
+  BelowAutograd below;
+  return op_norm_quantize().call(x, weight, eps, residual, gate, shift, scale, keep);
+}
+
+Tensor int8_linear_autograd(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                            const std::optional<Tensor>& bias, at::ScalarType dtype) {
+  no_gradient("int8_linear", {&scale, &weight_scale, &or_none(bias)});
+  BelowAutograd below;
+  return op_int8_linear().call(q, scale, weight, weight_scale, bias, dtype);
+}
+
+Tensor int8_gated_linear_autograd(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                                  const std::optional<Tensor>& bias, c10::string_view activation, at::ScalarType dtype) {
+  no_gradient("int8_gated_linear", {&scale, &weight_scale, &or_none(bias)});
+  BelowAutograd below;
+  return op_int8_gated_linear().call(q, scale, weight, weight_scale, bias, activation, dtype);
+}
+
 // Composite ops: they only open an autograd node around registered ops.
 std::tuple<Tensor, Tensor> read_with_residual(const Tensor& x, const Tensor& weight) {
   return pair(OpenFn::apply(x, weight));
@@ -2199,6 +2462,11 @@ TORCH_LIBRARY_IMPL(jit_thc, CUDA, m) {
   m.impl("gated_linear", gated_linear_cuda);
   m.impl("gated_linear_backward", gated_linear_backward_cuda);
   m.impl("axial_rope", axial_rope_cuda);
+  m.impl("quantize_rows", quantize_rows_cuda);
+  m.impl("dequantize_rows", dequantize_rows_cuda);
+  m.impl("norm_quantize", norm_quantize_cuda);
+  m.impl("int8_linear", int8_linear_cuda);
+  m.impl("int8_gated_linear", int8_gated_linear_cuda);
   m.impl("adamw_step", adamw_step_cuda);
   m.impl("adamw_state_values", adamw_state_values_cuda);
   m.impl("grad_norm", grad_norm_cuda);
@@ -2226,6 +2494,11 @@ static void autograd_kernels(torch::Library& m) {
   m.impl("gate_residual", gres_autograd);
   m.impl("gated_linear", gated_autograd);
   m.impl("axial_rope", axial_rope_autograd);
+  m.impl("quantize_rows", quantize_rows_autograd);
+  m.impl("dequantize_rows", dequantize_rows_autograd);
+  m.impl("norm_quantize", norm_quantize_autograd);
+  m.impl("int8_linear", int8_linear_autograd);
+  m.impl("int8_gated_linear", int8_gated_linear_autograd);
   for (const char* name : {"adamw_step", "adamw_state_values", "grad_norm"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }
 

@@ -653,6 +653,54 @@ size_t lthc_grad_norm_workspace_bytes(const int64_t* numels, int64_t count);
 int lthc_grad_norm(const void* const* grads, int g_dtype, const int64_t* numels, int64_t count, float* out,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * ROWS IN 8-BIT INTEGERS (no reference op).  For x [M, C] (x_dtype, rows x_ld
+ * elements apart, any address of an element):
+ *   s[m] = max(max_c |x[m,c]| / 127, 2^-126),  q[m,c] = rint(x[m,c] / s[m])
+ * q: int8 [M, Cp], Cp = C rounded up to a multiple of 16, zeros past C; scales:
+ * fp32 [M].  A value within 2^-21 (relative) of a tie goes to either side.  A row
+ * with a NaN or an infinity: s = NaN, q = 0.
+ * Back: out[m,c] = q[m,c] s[m] in out_dtype, [M, C]; q's rows q_ld elements apart, a
+ * multiple of 16 that is at least C.
+ */
+int lthc_quantize_rows(const void* x, int x_dtype, int64_t x_ld, int8_t* q, float* scales, int64_t M, int64_t C, void* stream);
+int lthc_dequantize_rows(const int8_t* q, int64_t q_ld, const float* scales, void* out, int out_dtype, int64_t M, int64_t C,
+                         void* stream);
+
+/*
+ * RMS NORM WITH THE RESIDUAL'S ADDITION AND AN OUTPUT IN 8 BITS (no reference op:
+ * dz = gate a, z + dz and modulate(norm(.)) of WorkspaceSharedAdaLNBranch.forward,
+ * local_thc.py:315-323, in front of an 8-bit layer).  For x [B N, C], N rows a sample:
+ *   u = gate[b] x,  t = residual + u,
+ *   y = t rsqrt(mean_c t^2 + eps) weight (1 + scale[b]) + shift[b],  (q, scales) = rows of y as above
+ * in fp32, nothing rounded in between.  residual (x_dtype), gate, and shift with scale
+ * may be NULL: 0, 1, and no modulation.  Rows are *_ld elements apart; gate_ld and mod_ld
+ * are between samples, 0 for one row for all.  kept [B N, C] (x_dtype): t (LTHC_KEEP_SUM) or
+ * u (LTHC_KEEP_UPDATE), rounded once; it may be the residual or x where these are dense.
+ */
+#define LTHC_KEEP_NONE 0
+#define LTHC_KEEP_SUM 1
+#define LTHC_KEEP_UPDATE 2
+int lthc_norm_quantize(const void* x, int x_dtype, int64_t x_ld, const void* residual, int64_t residual_ld, const void* gate,
+                       int gate_dtype, int64_t gate_ld, const void* weight, int weight_dtype, const void* shift, const void* scale,
+                       int mod_dtype, int64_t mod_ld, int keep, void* kept, int8_t* q, float* scales, int64_t B, int64_t N,
+                       int64_t C, float eps, void* stream);
+
+/*
+ * LINEAR LAYERS IN 8-BIT INTEGERS (no reference op: qkv, proj, w12 with its gate and w3 of
+ * the branch, local_thc.py:213-269).  For q int8 [M, K] with a scale for each row and
+ * weight int8 [N, K] with a scale for each row:
+ *   h[m,n] = (sum_k q[m,k] weight[n,k]) q_scales[m] w_scales[n] + bias[n],  y = h
+ * or, gated, weight [2F, K]: y[m,f] = act(h[m,f]) h[m,F+f].  Sums are exact (K up to 131056),
+ * the rest fp32, rounded once to y_dtype.  bias fp32 or NULL.  K and the row strides are
+ * multiples of 16, q and weight 16-byte aligned; any M, N and F.  y [M, N] ([M, F]).
+ */
+int lthc_int8_linear(const int8_t* q, int64_t q_ld, const float* q_scales, const int8_t* weight, int64_t w_ld, const float* w_scales,
+                     const float* bias, void* y, int y_dtype, int64_t M, int64_t N, int64_t K, void* stream);
+int lthc_int8_gated_linear(const int8_t* q, int64_t q_ld, const float* q_scales, const int8_t* weight, int64_t w_ld,
+                           const float* w_scales, const float* bias, int act, void* y, int y_dtype, int64_t M, int64_t F, int64_t K,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif
