@@ -180,10 +180,10 @@ def load() -> ctypes.CDLL:
         ],  # fmt: skip
         "lthc_adamw_state_values": [pp, pp, pp, pp, pp, pi, i64, vp],
         "lthc_grad_norm": [pp, ci, pi, i64, vp, vp, sz, vp],
-        "lthc_quantize_rows": [vp, ci, i64, vp, vp, i64, i64, vp],
+        "lthc_quantize_rows": [vp, ci, i64, vp, i64, vp, i64, i64, vp],
         "lthc_dequantize_rows": [vp, i64, vp, vp, ci, i64, i64, vp],
         "lthc_norm_quantize": [
-            vp, ci, i64, vp, i64, vp, ci, i64, vp, ci, vp, vp, ci, i64, ci, vp, vp, vp, i64, i64, i64, ctypes.c_float, vp,
+            vp, ci, i64, vp, i64, vp, ci, i64, vp, ci, vp, vp, ci, i64, ci, vp, vp, i64, vp, i64, i64, i64, ctypes.c_float, vp,
         ],  # fmt: skip
         "lthc_int8_linear": [vp, i64, vp, vp, i64, vp, vp, vp, ci, i64, i64, i64, vp],
         "lthc_int8_gated_linear": [vp, i64, vp, vp, i64, vp, vp, ci, vp, ci, i64, i64, i64, vp],

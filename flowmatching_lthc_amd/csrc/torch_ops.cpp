@@ -1145,22 +1145,32 @@ void check_channels(const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, name, " [..., C] with at least one channel expected, got ", shape(x));
 }
 
-std::tuple<Tensor, Tensor> empty_rows(const Tensor& x) {  // (q [..., up16(C)], scales [...])
-  auto sizes = x.sizes().vec();
-  sizes.back() = up16(sizes.back());
-  return {at::empty(sizes, x.options().dtype(at::kChar)), fp32_like(x.sizes().slice(0, x.dim() - 1), x)};
-}
+// Elements between the rows of new 8-bit rows of Cp: whole lines of memory, but for short rows.
+int64_t row_pitch(int64_t cp) { return cp < 512 ? cp : (cp + 127) / 128 * 128; }
+
+struct NewRows {
+  Tensor q, s;  // [..., up16(C)], [...]
+  int64_t ld;
+  explicit NewRows(const Tensor& x) {
+    auto sizes = x.sizes().vec();
+    const int64_t cp = up16(sizes.back());
+    ld = sizes.back() = row_pitch(cp);
+    q = at::empty(sizes, x.options().dtype(at::kChar));
+    if (ld != cp) q = q.narrow(-1, 0, cp);
+    s = fp32_like(x.sizes().slice(0, x.dim() - 1), x);
+  }
+};
 
 std::tuple<Tensor, Tensor> quantize_rows_cuda(const Tensor& x_) {
   on_gpu(x_);
   check_channels(x_, "x");
   const int dt = code(x_);
   const Rows x(x_);
-  auto [q, s] = empty_rows(x_);
+  const NewRows o(x_);
   const Launch l(x_);
-  check(lthc_quantize_rows(data(x.t), dt, x.ld, q.data_ptr<int8_t>(), s.data_ptr<float>(), s.numel(), x_.size(-1), l.stream),
+  check(lthc_quantize_rows(data(x.t), dt, x.ld, o.q.data_ptr<int8_t>(), o.ld, o.s.data_ptr<float>(), o.s.numel(), x_.size(-1), l.stream),
         "lthc_quantize_rows");
-  return {q, s};
+  return {o.q, o.s};
 }
 
 void check_scales(const Tensor& q, const Tensor& s, const char* name) {
@@ -1234,19 +1244,19 @@ std::tuple<Tensor, Tensor, Tensor> norm_quantize_cuda(const Tensor& x_, const Te
     }
   }
   const Tensor w = (known_dtype(weight) ? weight : weight.to(at::kFloat)).contiguous();
-  auto [q, s] = empty_rows(x_);
+  const NewRows o(x_);
   Tensor out = kept == LTHC_KEEP_NONE ? at::empty({0}, x_.options()) : at::empty(x_.sizes(), x_.options());
   // [B, N, C]: N rows a sample; otherwise one sample
-  const int64_t n = x_.dim() == 3 ? x_.size(1) : s.numel(), b = x_.dim() == 3 ? x_.size(0) : 1;
+  const int64_t n = x_.dim() == 3 ? x_.size(1) : o.s.numel(), b = x_.dim() == 3 ? x_.size(0) : 1;
   const auto at = [](const Tensor& t) { return t.defined() ? data(t) : nullptr; };
   const auto type = [](const Tensor& t) { return t.defined() ? code(t) : LTHC_F32; };
   const Launch l(x_);
   check(lthc_norm_quantize(data(x.t), dt, x.ld, given(residual_) ? data(residual.t) : nullptr, residual.ld, at(gate.first),
                            type(gate.first), gate.second, data(w), code(w), at(shift.first), at(scale.first), type(shift.first),
-                           shift.second, kept, kept ? data(out) : nullptr, q.data_ptr<int8_t>(), s.data_ptr<float>(), b, n, c,
+                           shift.second, kept, kept ? data(out) : nullptr, o.q.data_ptr<int8_t>(), o.ld, o.s.data_ptr<float>(), b, n, c,
                            static_cast<float>(eps), l.stream),
         "lthc_norm_quantize");
-  return {out, q, s};
+  return {out, o.q, o.s};
 }
 
 struct Int8Operands {

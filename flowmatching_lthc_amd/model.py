@@ -30,6 +30,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from . import ops, ops_branch
 from .local_thc import LayerLocalWrite, SharedLocalRead, overridden
+from .quantized import Int8Linear, QuantizedRows, norm_rows
 
 
 def modulate(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -326,9 +327,10 @@ class WorkspaceAttention(nn.Module):
             and ops_branch.attention_supported(qkv5)
         )
 
-    def forward(self, x: torch.Tensor, rope: VisionRotaryEmbeddingFast) -> torch.Tensor:
-        b, n, c = x.shape
+    def forward(self, x: torch.Tensor | QuantizedRows, rope: VisionRotaryEmbeddingFast) -> torch.Tensor:
         qkv = self.qkv(x)
+        b, n = x.shape[:2]
+        c = self.num_heads * self.head_dim
         if self._fused_qk(qkv, rope):
             qkv5 = qkv.view(b, n, 3, self.num_heads, self.head_dim)
             if self._fused_attn(qkv5):
@@ -388,7 +390,9 @@ class SwiGLUFFN(nn.Module):
             return None
         return ops_branch.gated_linear(x, w, b)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor | QuantizedRows) -> torch.Tensor:
+        if type(self.w12) is Int8Linear and not _watched(self.w12):
+            return self.w3(self.ffn_dropout(self.w12.gated(x, "silu")))
         act = self._fused_act(x)
         if act is not None:
             return self.w3(self.ffn_dropout(act))
@@ -399,6 +403,24 @@ class SwiGLUFFN(nn.Module):
             gate, value = h.chunk(2, dim=-1)
             act = F.silu(gate) * value
         return self.w3(self.ffn_dropout(act))
+
+
+def _watched(m: nn.Module) -> bool:
+    """Whether something else than the call sees or replaces what module m is called with."""
+    return bool(m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__) or nn.modules.module._has_any_global_hook()
+
+
+def _takes_rows(module: nn.Module, name: str, norm: nn.Module, x: torch.Tensor) -> bool:
+    """Whether `norm` on x can hand `module` (attention or feed-forward), whose first layer is `name`, its output as 8-bit
+    rows: an Int8Linear there, modules of this package that nothing watches, a GPU tensor of the operators' dtypes."""
+    layer = module._modules.get(name) if type(module) in (WorkspaceAttention, SwiGLUFFN) else None
+    return (
+        type(layer) is Int8Linear
+        and type(norm) is RMSNorm
+        and not (_watched(layer) or _watched(module))
+        and x.is_cuda
+        and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
+    )
 
 
 class WorkspaceSharedAdaLNBranch(nn.Module):
@@ -424,14 +446,28 @@ class WorkspaceSharedAdaLNBranch(nn.Module):
 
     def forward(self, z: torch.Tensor, t6: torch.Tensor, rope: VisionRotaryEmbeddingFast) -> torch.Tensor:
         sh_a, sc_a, g_a, sh_m, sc_m, g_m = t6.chunk(6, dim=-1)
-        a = self.attn(norm_modulate(self.norm1, z, sh_a, sc_a), rope)
+        a = self.attn(self.attention_input(z, sh_a, sc_a), rope)
         if self.fused_gates(z, a, t6):
             # d_attn = g_a * a, z + d_attn and its pre-norm in one HIP pass; d_attn + g_m * mlp in another
-            d_attn, h = ops_branch.gate_add_norm_modulate(z, a, g_a, self.norm2.weight, sh_m, sc_m, self.norm2.eps)
+            d_attn, h = self.mlp_input(z, a, g_a, sh_m, sc_m)
             return ops_branch.gate_residual(d_attn, g_m, self.mlp(h))
         d_attn = g_a.unsqueeze(1) * a
         d_mlp = g_m.unsqueeze(1) * self.mlp(norm_modulate(self.norm2, z + d_attn, sh_m, sc_m))
         return d_attn + d_mlp
+
+    def attention_input(self, z: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor | QuantizedRows:
+        """The branch's first pre-norm, as 8-bit rows where qkv takes them."""
+        if _takes_rows(self.attn, "qkv", self.norm1, z) and z.dtype == shift.dtype:
+            return norm_rows(self.norm1, z, shift, scale)[1]
+        return norm_modulate(self.norm1, z, shift, scale)
+
+    def mlp_input(
+        self, z: torch.Tensor, a: torch.Tensor, gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor
+    ) -> tuple[torch.Tensor, torch.Tensor | QuantizedRows]:
+        """(gate * a, the second pre-norm of z + gate * a), the latter as 8-bit rows where w12 takes them."""
+        if _takes_rows(self.mlp, "w12", self.norm2, z):
+            return norm_rows(self.norm2, a, shift, scale, z, gate, "update")
+        return ops_branch.gate_add_norm_modulate(z, a, gate, self.norm2.weight, shift, scale, self.norm2.eps)
 
     @staticmethod
     def fused_gates(z: torch.Tensor, a: torch.Tensor, t6: torch.Tensor) -> bool:
@@ -439,15 +475,15 @@ class WorkspaceSharedAdaLNBranch(nn.Module):
         return z.is_cuda and z.dim() == 3 and a.dtype == z.dtype == t6.dtype and z.shape[-1] % 8 == 0 and z.shape[-1] <= 2048
 
     def parts(
-        self, z: torch.Tensor, t6: torch.Tensor, rope: VisionRotaryEmbeddingFast, y1: torch.Tensor | None = None
+        self, z: torch.Tensor, t6: torch.Tensor, rope: VisionRotaryEmbeddingFast, y1: torch.Tensor | QuantizedRows | None = None
     ) -> tuple[torch.Tensor, torch.Tensor] | None:
         """(g_a * attn, mlp output): forward() without its last gated residual, or None where the gated residuals
         are not HIP passes.  y1: this branch's first pre-norm output when the caller has computed it."""
         sh_a, sc_a, g_a, sh_m, sc_m, _ = t6.chunk(6, dim=-1)
-        a = self.attn(y1 if y1 is not None else norm_modulate(self.norm1, z, sh_a, sc_a), rope)
+        a = self.attn(y1 if y1 is not None else self.attention_input(z, sh_a, sc_a), rope)
         if not self.fused_gates(z, a, t6):
             return None
-        d_attn, h = ops_branch.gate_add_norm_modulate(z, a, g_a, self.norm2.weight, sh_m, sc_m, self.norm2.eps)
+        d_attn, h = self.mlp_input(z, a, g_a, sh_m, sc_m)
         return d_attn, self.mlp(h)
 
 
@@ -952,8 +988,13 @@ class SharedReadLocalTHCSharedAdaLNJiT(BatchedWeightCast, nn.Module):
                 if gammas is None:
                     return None
             if i + 1 < nb:
-                n1 = self.blocks[i + 1].branch.norm1
-                dz, z, y1 = ops_branch.block_tail(z, d_attn, g_m, mo, gammas[i], n1.weight, sh_a, sc_a, n1.eps)
+                following = self.blocks[i + 1].branch
+                n1 = following.norm1
+                if _takes_rows(following.attn, "qkv", n1, z):
+                    dz = ops_branch.gate_residual(d_attn, g_m, mo)
+                    z, y1 = norm_rows(n1, dz, sh_a, sc_a, z, gammas[i], "sum")
+                else:
+                    dz, z, y1 = ops_branch.block_tail(z, d_attn, g_m, mo, gammas[i], n1.weight, sh_a, sc_a, n1.eps)
             else:  # the last step's Z_L feeds nothing
                 dz = ops_branch.gate_residual(d_attn, g_m, mo)
             dz_list.append(dz)

@@ -30,6 +30,21 @@ def padded(channels: int) -> int:
     return -(-channels // 16) * 16
 
 
+def _new_rows(x: Tensor) -> tuple[Tensor, Tensor]:
+    """(q, scale) for the rows of x: rows of 512 elements and more begin at whole lines of memory, 128 bytes."""
+    c = padded(x.shape[-1])
+    q = x.new_empty((*x.shape[:-1], c if c < 512 else -(-c // 128) * 128), dtype=torch.int8)
+    return q[..., :c], x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+def whole_lines(q: Tensor) -> Tensor:
+    """8-bit rows [N, K] in the layout that quantize_rows gives them on the GPU: themselves, or a copy."""
+    if not q.is_cuda or padded(q.shape[1]) != q.shape[1]:
+        return q
+    to, _ = _new_rows(q)
+    return q if q.stride() == to.stride() else to.copy_(q)
+
+
 # ---------------------------------------------------------------------------
 # eager restatements: what the kernels' values are compared with
 # ---------------------------------------------------------------------------
@@ -73,14 +88,14 @@ def int8_gated_linear_eager(
 @torch.library.custom_op("jit_thc::quantize_rows", mutates_args=())
 def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
     """(q, scale) of x [..., C], fp32, bf16 or fp16: scale = max(max |x| / 127, 2^-126) of each row, q = rint(x / scale) as
-    int8 [..., padded(C)], zeros past C.  A value within 2^-21 (relative) of a tie goes to either side.  A row with a NaN or
+    int8 [..., padded(C)], zeros past C; rows of 512 elements and more lie a multiple of 128 apart.  A value within 2^-21 (relative) of a tie goes to either side.  A row with a NaN or
     an infinity has the scale NaN and q 0."""
     _refuse(x)
 
 
 @_fake(quantize_rows)
 def _(x):
-    return x.new_empty((*x.shape[:-1], padded(x.shape[-1])), dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return _new_rows(x)
 
 
 @torch.library.custom_op("jit_thc::dequantize_rows", mutates_args=())
@@ -110,7 +125,7 @@ def norm_quantize(
 @_fake(norm_quantize)
 def _(x, weight, eps, residual=None, gate=None, shift=None, scale=None, keep="none"):
     kept = x.new_empty((0,) if keep == "none" else x.shape)
-    return kept, x.new_empty((*x.shape[:-1], padded(x.shape[-1])), dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return kept, *_new_rows(x)
 
 
 # ---------------------------------------------------------------------------

@@ -1,0 +1,110 @@
+"""The workspace branch's linear layers in 8-bit integers, for inference.
+
+``quantize_branches(model)`` replaces qkv, proj, w12 and w3 (local_thc.py:213-269) of every branch of a model by
+``Int8Linear``: weights in 8 bits with a scale for each channel, laid out once; activations in 8 bits with a scale for each
+token, formed on the way.  A branch whose layers have that form runs the 8-bit operators where its elementwise chains feed
+them: its norms write 8-bit rows (``ops_int8.norm_quantize``), w12 with the activation is one product
+(``ops_int8.int8_gated_linear``).  Everything around the branches stays as it is.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import ops_int8
+
+
+class QuantizedRows(NamedTuple):
+    """8-bit rows with their scales, and the dtype of the activations that they stand for."""
+
+    values: Tensor
+    scale: Tensor
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+
+class Int8Linear(nn.Module):
+    """nn.Linear for inference on 8-bit rows: weight int8 [out, in rounded up to a multiple of 16], weight_scale and bias fp32.
+
+    forward takes activations (quantised here) or QuantizedRows and returns the activations' dtype (autocast's in its
+    region).  weight_scale and bias stay fp32 when the module is converted to another dtype."""
+
+    def __init__(self, weight: Tensor, weight_scale: Tensor, bias: Tensor | None, in_features: int) -> None:
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = weight.shape[0]
+        self.register_buffer("weight", ops_int8.whole_lines(weight))
+        self.register_buffer("weight_scale", weight_scale)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, layer: nn.Linear) -> Int8Linear:
+        w = layer.weight.detach()
+        q, scale = ops_int8.quantize_rows(w) if w.is_cuda else ops_int8.quantize_rows_eager(w)
+        return cls(q, scale, None if layer.bias is None else layer.bias.detach().float().clone(), layer.in_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+    def _apply(self, fn, recurse: bool = True):
+        kept = {n: b for n, b in (("weight_scale", self.weight_scale), ("bias", self.bias)) if b is not None}
+        super()._apply(fn, recurse)
+        for n, b in kept.items():  # where fn only changed the dtype, the fp32 values themselves
+            moved = getattr(self, n)
+            if moved.dtype != torch.float32:
+                setattr(self, n, b.to(moved.device))
+        self.weight = ops_int8.whole_lines(self.weight)
+        return self
+
+    def rows(self, x: Tensor | QuantizedRows) -> QuantizedRows:
+        if isinstance(x, QuantizedRows):
+            return x
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        return QuantizedRows(*ops_int8.quantize_rows(x), dtype)
+
+    def forward(self, x: Tensor | QuantizedRows) -> Tensor:
+        q, scale, dtype = self.rows(x)
+        return ops_int8.int8_linear(q, scale, self.weight, self.weight_scale, self.bias, dtype)
+
+    def gated(self, x: Tensor | QuantizedRows, activation: str) -> Tensor:
+        """act(g) * u of this layer's two halves (g, u)."""
+        q, scale, dtype = self.rows(x)
+        return ops_int8.int8_gated_linear(q, scale, self.weight, self.weight_scale, self.bias, activation, dtype)
+
+
+def norm_rows(
+    norm: nn.Module, x: Tensor, shift: Tensor, scale: Tensor, residual: Tensor | None = None, gate: Tensor | None = None, keep: str = "none"
+) -> tuple[Tensor, QuantizedRows]:
+    """(kept, modulate(norm(residual + gate * x), shift, scale) as 8-bit rows): ops_int8.norm_quantize of an RMSNorm."""
+    kept, q, s = ops_int8.norm_quantize(x, norm.weight, norm.eps, residual, gate, shift, scale, keep)
+    return kept, QuantizedRows(q, s, x.dtype)
+
+
+def quantize_branches(model: nn.Module) -> nn.Module:
+    """Replaces the linear layers of every workspace branch of `model` by Int8Linear, in place, and returns the model.
+
+    For inference: load the weights first (the state dict holds 8-bit weights afterwards), call the model under
+    torch.no_grad().  A layer that is not a plain linear layer (hooks, a parametrization, another class) is refused."""
+    from .model import SwiGLUFFN, WorkspaceAttention, _plain_projection
+
+    found = [(m, n) for m in model.modules() if isinstance(m, WorkspaceAttention) for n in ("qkv", "proj")]
+    found += [(m, n) for m in model.modules() if isinstance(m, SwiGLUFFN) for n in ("w12", "w3")]
+    if not found:
+        raise ValueError("the model has no workspace branch")
+    for m, n in found:
+        layer = getattr(m, n)
+        if not (type(layer) is Int8Linear or _plain_projection(layer)):
+            raise ValueError(f"{type(m).__name__}.{n} is not a plain linear layer: {type(layer).__name__}")
+    for m, n in found:
+        layer = getattr(m, n)
+        if type(layer) is not Int8Linear:
+            setattr(m, n, Int8Linear.from_linear(layer))
+    return model

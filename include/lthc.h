@@ -657,13 +657,14 @@ int lthc_grad_norm(const void* const* grads, int g_dtype, const int64_t* numels,
  * ROWS IN 8-BIT INTEGERS (no reference op).  For x [M, C] (x_dtype, rows x_ld
  * elements apart, any address of an element):
  *   s[m] = max(max_c |x[m,c]| / 127, 2^-126),  q[m,c] = rint(x[m,c] / s[m])
- * q: int8 [M, Cp], Cp = C rounded up to a multiple of 16, zeros past C; scales:
- * fp32 [M].  A value within 2^-21 (relative) of a tie goes to either side.  A row
+ * q: int8 [M, Cp], Cp = C rounded up to a multiple of 16, zeros past C, rows q_ld
+ * elements apart (a multiple of 16; of 128 where the products should load whole lines);
+ * scales: fp32 [M].  A value within 2^-21 (relative) of a tie goes to either side.  A row
  * with a NaN or an infinity: s = NaN, q = 0.
- * Back: out[m,c] = q[m,c] s[m] in out_dtype, [M, C]; q's rows q_ld elements apart, a
- * multiple of 16 that is at least C.
+ * Back: out[m,c] = q[m,c] s[m] in out_dtype, [M, C].
  */
-int lthc_quantize_rows(const void* x, int x_dtype, int64_t x_ld, int8_t* q, float* scales, int64_t M, int64_t C, void* stream);
+int lthc_quantize_rows(const void* x, int x_dtype, int64_t x_ld, int8_t* q, int64_t q_ld, float* scales, int64_t M, int64_t C,
+                       void* stream);
 int lthc_dequantize_rows(const int8_t* q, int64_t q_ld, const float* scales, void* out, int out_dtype, int64_t M, int64_t C,
                          void* stream);
 
@@ -683,8 +684,8 @@ int lthc_dequantize_rows(const int8_t* q, int64_t q_ld, const float* scales, voi
 #define LTHC_KEEP_UPDATE 2
 int lthc_norm_quantize(const void* x, int x_dtype, int64_t x_ld, const void* residual, int64_t residual_ld, const void* gate,
                        int gate_dtype, int64_t gate_ld, const void* weight, int weight_dtype, const void* shift, const void* scale,
-                       int mod_dtype, int64_t mod_ld, int keep, void* kept, int8_t* q, float* scales, int64_t B, int64_t N,
-                       int64_t C, float eps, void* stream);
+                       int mod_dtype, int64_t mod_ld, int keep, void* kept, int8_t* q, int64_t q_ld, float* scales, int64_t B,
+                       int64_t N, int64_t C, float eps, void* stream);
 
 /*
  * LINEAR LAYERS IN 8-BIT INTEGERS (no reference op: qkv, proj, w12 with its gate and w3 of

@@ -45,6 +45,7 @@ def test_quantize_rows(dtype, m, c):
     x = randn(m, c, dtype=dtype) * 3
     q, s = ops_int8.quantize_rows(x)
     check_rows(q, s, x.double(), torch.zeros(m, 1, device=DEV, dtype=torch.float64))
+    assert q.stride() == ops_int8.quantize_rows(x.to("meta"))[0].stride()
     # the quotient rounded once: 53 bits hold enough of it for the second rounding, to 24, to be its only one
     assert torch.equal(s, (x.double().abs().amax(-1) / 127).float().clamp(min=ops_int8.TINY))
 

@@ -1,0 +1,251 @@
+"""The branch's layers in 8 bits: the layer, the models' inference on it, captured and compiled."""
+
+import copy
+import io
+
+import pytest
+import torch
+import torch.nn as nn
+
+from flowmatching_lthc_amd import model as M
+from flowmatching_lthc_amd import ops_branch, ops_int8
+from flowmatching_lthc_amd.model_triangular import PerBlock_JiT_models
+from flowmatching_lthc_amd.quantized import Int8Linear, QuantizedRows, quantize_branches
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def linear(k, n, dtype=torch.float32, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    layer = M.CastLinear(k, n)
+    with torch.no_grad():
+        layer.weight.copy_(torch.randn(n, k, generator=gen) * k**-0.5)
+        layer.bias.copy_(torch.randn(n, generator=gen))
+    return layer.to(DEV, dtype)
+
+
+def randn(*shape, dtype=torch.bfloat16, seed=0):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 768, 96), (5, 100, 33), (130, 2730, 70)])
+@torch.no_grad()
+def test_layer_is_within_its_roundings_of_the_linear_layer(dtype, m, k, n):
+    layer = linear(k, n)
+    q = Int8Linear.from_linear(layer)
+    x = randn(2, m, k, dtype=dtype)
+    y = q(x)
+    assert y.dtype == dtype and y.shape == (2, m, n)
+    # an operand is off by half its row's step (and 2^-17 of one, where the reciprocal's rounding moves a value over a tie)
+    x64, w64 = x.double(), layer.weight.double()
+    dx = (0.5 + 2.0**-17) * x64.abs().amax(-1, keepdim=True) / 127
+    dw = (0.5 + 2.0**-17) * w64.abs().amax(-1) / 127
+    want = x64 @ w64.t().contiguous() + layer.bias.double()
+    bound = dx * w64.abs().sum(-1) + x64.abs().sum(-1, keepdim=True) * dw + k * dx * dw
+    bound = bound * (1 + 2.0**-20) + (torch.finfo(dtype).eps / 2 + 2.0**-21) * (want.abs() + bound) + 2.0**-21 * layer.bias.double().abs()
+    assert bool(((y.double() - want).abs() <= bound).all())
+
+
+@torch.no_grad()
+def test_layer_keeps_its_numbers_through_conversions_copies_and_files():
+    cpu = Int8Linear.from_linear(linear(2730, 40).cpu())
+    layer = copy.deepcopy(cpu).to(DEV)
+    assert layer.weight.shape == (40, 2736) and layer.weight.stride() == (2816, 1)
+    x = randn(3, 2730)
+    want = layer(x)
+    for other in (copy.deepcopy(layer).half(), copy.deepcopy(layer).to(torch.bfloat16), copy.deepcopy(cpu).to(DEV, torch.float16), copy.deepcopy(layer).cpu().to(DEV)):
+        assert other.weight_scale.dtype == torch.float32 and other.bias.dtype == torch.float32 and other.weight.dtype == torch.int8
+        assert torch.equal(other(x), want)
+    file = io.BytesIO()
+    torch.save(layer.state_dict(), file)
+    file.seek(0)
+    new = Int8Linear.from_linear(linear(2730, 40, seed=5))
+    new.load_state_dict(torch.load(file, weights_only=True))
+    assert torch.equal(new(x), want)
+    with torch.autocast("cuda", torch.float16):
+        assert layer(x.float()).dtype == torch.float16
+
+
+def branch(dim=256, heads=4, seed=1, cls=M.WorkspaceSharedAdaLNBranch):
+    torch.manual_seed(seed)
+    b = cls(dim, heads)
+    with torch.no_grad():
+        for n, p in b.named_parameters():
+            p.copy_(1 + 0.1 * torch.randn_like(p) if "norm" in n else torch.randn_like(p) * (p.shape[-1] ** -0.5))
+    return b.to(DEV).eval()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@torch.no_grad()
+def test_branch_runs_the_8_bit_operators(dtype):
+    b = quantize_branches(branch())
+    b = b.to(dtype)
+    rope = M.VisionRotaryEmbeddingFast(32, 8).to(DEV)
+    z, t6 = randn(3, 64, 256, dtype=dtype), 0.3 * randn(3, 6 * 256, dtype=dtype, seed=3)
+    got = b(z, t6, rope)
+    sh_a, sc_a, g_a, sh_m, sc_m, g_m = t6.chunk(6, -1)
+
+    def layer(x, which, gated=False):
+        q, s = x if isinstance(x, tuple) else ops_int8.quantize_rows(x)
+        op = (lambda *a: ops_int8.int8_gated_linear(*a, "silu", dtype)) if gated else (lambda *a: ops_int8.int8_linear(*a, dtype))
+        return op(q, s, which.weight, which.weight_scale, which.bias)
+
+    qkv = layer(ops_int8.norm_quantize(z, b.norm1.weight, 1e-6, None, None, sh_a, sc_a)[1:], b.attn.qkv).view(3, 64, 3, 4, 64)
+    if dtype == torch.float32:
+        q, k = ops_branch.qk_norm_rope(qkv, b.attn.q_norm.weight, b.attn.k_norm.weight, rope.freqs_cos, rope.freqs_sin, 1e-6)
+        with b.attn._backends():
+            o = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), qkv[:, :, 2].transpose(1, 2)).transpose(1, 2)
+    else:
+        o = ops_branch.qk_norm_rope_attention(qkv, b.attn.q_norm.weight, b.attn.k_norm.weight, *rope.tables(dtype), 1e-6)
+    a = layer(o.reshape(3, 64, 256), b.attn.proj)
+    d, q, s = ops_int8.norm_quantize(a, b.norm2.weight, 1e-6, z, g_a, sh_m, sc_m, "update")
+    want = ops_branch.gate_residual(d, g_m, layer(layer((q, s), b.mlp.w12, gated=True), b.mlp.w3))
+    assert got.dtype == dtype and torch.equal(got, want)
+
+
+@torch.no_grad()
+def test_branch_with_watched_modules_quantises_in_the_layer():
+    b = quantize_branches(branch())
+    rope = M.VisionRotaryEmbeddingFast(32, 8).to(DEV)
+    z, t6 = randn(2, 64, 256, dtype=torch.float32), 0.3 * randn(2, 6 * 256, dtype=torch.float32, seed=3)
+    want = b(z, t6, rope)
+    seen = []
+    for m in (b.attn.qkv, b.mlp.w12, b.attn, b.mlp):
+        handle = m.register_forward_pre_hook(lambda mod, args: seen.append(type(args[0])))
+        got = b(z, t6, rope)
+        handle.remove()
+        # the same function with the norm's output stored on the way, in fp32 here: a few values pass to the next step
+        assert float((got - want).abs().max()) <= 2.0**-6 * float(want.abs().max())
+    assert len(seen) == 4 and QuantizedRows not in seen
+
+
+def built(name):
+    torch.manual_seed(0)
+    return M.randomize_parameters(M.build_model(name)).to(DEV).eval()
+
+
+def inputs(seed, size=256, b=2):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s: torch.rand(s, generator=gen, device=DEV)  # noqa: E731
+    return r(b, 3, size, size) * 2 - 1, r(b), torch.randint(0, 1000, (b,), generator=gen, device=DEV)
+
+
+NAMES = [
+    "lthc_b4_velocity",
+    "SharedRead-LocalTHC-SharedAdaLN-JiT-B/4",
+    "local_thc_v2_fused_final12_shared_adaln_b4",
+    "local_thc_v2_fused_final12_adaln_b4",
+    next(iter(PerBlock_JiT_models)),
+]
+
+
+@pytest.mark.parametrize("name", NAMES)
+@torch.no_grad()
+def test_models_run_in_8_bits(name):
+    model = built(name)
+    x = inputs(1)
+    with torch.autocast("cuda", torch.bfloat16):
+        before = model(*x)
+        assert quantize_branches(model) is model
+        after = model(*x)
+    kinds = {type(m) for m in model.modules()}
+    assert Int8Linear in kinds and after.shape == before.shape and after.dtype == before.dtype
+    # 8-bit operands are off by about 0.5 / 127 x 4 / sqrt(3) of their size, 0.01; a branch's update, a part of the output, by
+    # the four products' together
+    assert float((after - before).float().norm()) <= 0.1 * float(before.float().norm())
+    assert not torch.equal(after, before)
+
+
+@torch.no_grad()
+def test_model_captured_and_replayed():
+    model = quantize_branches(built("lthc_b4_velocity"))
+    static = [t.clone() for t in inputs(0)]
+
+    def call():
+        with torch.autocast("cuda", torch.bfloat16):
+            return model(*static)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for seed in (5, 6, 5, 7):
+        for t, new in zip(static, inputs(seed)):
+            t.copy_(new)
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call())
+
+
+@torch.no_grad()
+def test_two_captured_graphs_and_eager_calls_share_nothing():
+    w, v = ops_int8.quantize_rows(randn(512, 768, dtype=torch.float32))
+    xs = [randn(200, 768, seed=i) for i in range(2)]
+
+    def call(x):
+        kept, q, s = ops_int8.norm_quantize(x, torch.ones(768, device=DEV), 1e-6, x, keep="sum")
+        return kept, ops_int8.int8_gated_linear(q, s, w, v), ops_int8.int8_linear(q, s, w, v, None, torch.float32)
+
+    want = [call(x) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(3):
+        for g, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = call(xs[0])
+        torch.cuda.synchronize()
+        for got, ref in [*zip(outs, want), (eager, want[0])]:
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@torch.no_grad()
+def test_operators_in_a_compiled_function():
+    layer, norm = Int8Linear.from_linear(linear(256, 96)), M.RMSNorm(256).to(DEV)
+    gated = Int8Linear.from_linear(linear(256, 128, seed=2))
+
+    def f(x, shift, scale):
+        kept, q, s = ops_int8.norm_quantize(x, norm.weight, norm.eps, x, None, shift, scale, "sum")
+        rows = QuantizedRows(q, s, x.dtype)
+        return kept, layer(rows), gated.gated(rows, "gelu"), ops_int8.dequantize_rows(q, s, 256, torch.float32)
+
+    x, sh, sc = randn(2, 30, 256), randn(2, 256, seed=1), randn(2, 256, seed=2)
+    got = torch.compile(f, fullgraph=True)(x, sh, sc)
+    for a, b in zip(got, f(x, sh, sc)):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_a_recorded_call_is_refused():
+    b = quantize_branches(branch())
+    rope = M.VisionRotaryEmbeddingFast(32, 8).to(DEV)
+    z, t6 = randn(1, 64, 256, dtype=torch.float32), randn(1, 6 * 256, dtype=torch.float32)
+    with pytest.raises(ValueError, match="no_grad"):
+        b(z, t6, rope)
+    with torch.inference_mode():
+        b(z, t6, rope)
+
+
+def test_layers_that_are_something_else_are_refused():
+    b = branch()
+    b.mlp.w3.register_forward_hook(lambda *a: None)
+    with pytest.raises(ValueError, match="w3"):
+        quantize_branches(b)
+    assert type(b.attn.qkv) is M.CastLinear
+    with pytest.raises(ValueError, match="no workspace branch"):
+        quantize_branches(nn.Linear(3, 3))

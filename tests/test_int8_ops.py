@@ -20,19 +20,21 @@ def refused(rc, code, text):
 def test_row_entry_points_refuse_bad_arguments():
     lib = _abi.load()
     inv, uns = _abi.ERR_INVALID, _abi.ERR_UNSUPPORTED
-    refused(lib.lthc_quantize_rows(FAKE, 7, 8, FAKE, FAKE, 2, 8, None), inv, "dtype")
-    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, FAKE, 2, 0, None), inv, "positive")
-    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, FAKE, -1, 8, None), inv, "positive")
-    refused(lib.lthc_quantize_rows(FAKE, 1, -8, FAKE, FAKE, 2, 8, None), inv, "stride")
-    refused(lib.lthc_quantize_rows(ODD, 1, 8, FAKE, FAKE, 2, 8, None), inv, "misaligned")
-    refused(lib.lthc_quantize_rows(FAKE, 1, 8, ODD, FAKE, 2, 8, None), inv, "16-byte")
-    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, None, 2, 8, None), inv, "scales")
-    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, FAKE, 2, (1 << 28) + 1, None), uns, "channels")
+    refused(lib.lthc_quantize_rows(FAKE, 7, 8, FAKE, 16, FAKE, 2, 8, None), inv, "dtype")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, 16, FAKE, 2, 0, None), inv, "positive")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, 16, FAKE, -1, 8, None), inv, "positive")
+    refused(lib.lthc_quantize_rows(FAKE, 1, -8, FAKE, 16, FAKE, 2, 8, None), inv, "stride")
+    refused(lib.lthc_quantize_rows(ODD, 1, 8, FAKE, 16, FAKE, 2, 8, None), inv, "misaligned")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 8, ODD, 16, FAKE, 2, 8, None), inv, "16-byte")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, 16, None, 2, 8, None), inv, "scales")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 8, FAKE, 16, FAKE, 2, (1 << 28) + 1, None), uns, "channels")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 24, FAKE, 16, FAKE, 2, 24, None), inv, "multiple of 16")
+    refused(lib.lthc_quantize_rows(FAKE, 1, 24, FAKE, 40, FAKE, 2, 24, None), inv, "multiple of 16")
     refused(lib.lthc_dequantize_rows(FAKE, 24, FAKE, FAKE, 0, 2, 20, None), inv, "multiple of 16")
     refused(lib.lthc_dequantize_rows(FAKE, 16, FAKE, FAKE, 0, 2, 20, None), inv, "multiple of 16")
     norm = lambda **k: lib.lthc_norm_quantize(*({  # noqa: E731
         "x": FAKE, "dt": 1, "ld": 8, "r": FAKE, "rld": 8, "g": FAKE, "gdt": 1, "gld": 8, "w": FAKE, "wdt": 0, "sh": FAKE, "sc": FAKE,
-        "mdt": 1, "mld": 8, "keep": 1, "kept": FAKE, "q": FAKE, "s": FAKE, "b": 2, "n": 3, "c": 8, "eps": 1e-6, "st": None,
+        "mdt": 1, "mld": 8, "keep": 1, "kept": FAKE, "q": FAKE, "qld": 16, "s": FAKE, "b": 2, "n": 3, "c": 8, "eps": 1e-6, "st": None,
     } | k).values())  # fmt: skip
     refused(norm(w=None), inv, "weight")
     refused(norm(sh=None), inv, "together")
@@ -98,6 +100,8 @@ def test_shapes_of_fake_tensors():
         kept, q, s = ops_int8.norm_quantize(x, x[0, 0].float(), 1e-6, x, keep="sum")
         assert kept.shape == x.shape and kept.dtype == x.dtype and q.shape == (2, 5, 48)
         assert ops_int8.norm_quantize(x, x[0, 0], 1e-6)[0].shape == (0,)
+        long, _ = ops_int8.quantize_rows(torch.empty(3, 2, 2730, device="cuda"))
+        assert long.shape == (3, 2, 2736) and long.stride() == (5632, 2816, 1)
         w, v = torch.empty(6, 48, device="cuda", dtype=torch.int8), torch.empty(6, device="cuda")
         y = ops_int8.int8_linear(q, s, w, v, None, torch.float32)
         assert y.shape == (2, 5, 6) and y.dtype == torch.float32
