@@ -1135,7 +1135,7 @@ struct Rows {
 // The same for int8 rows, which the products load in aligned pieces of 16.
 struct Int8Rows : Rows {
   explicit Int8Rows(const Tensor& x) : Rows(x) {
-    if (ld % 16 == 0 && aligned(t, 16)) return;
+    if (ld % 16 == 0 && ld <= (1 << 22) && aligned(t, 16)) return;
     t = t.clone(at::MemoryFormat::Contiguous);
     ld = t.size(-1);
   }

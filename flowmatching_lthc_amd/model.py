@@ -329,7 +329,7 @@ class WorkspaceAttention(nn.Module):
 
     def forward(self, x: torch.Tensor | QuantizedRows, rope: VisionRotaryEmbeddingFast) -> torch.Tensor:
         qkv = self.qkv(x)
-        b, n = x.shape[:2]
+        b, n = qkv.shape[:2]
         c = self.num_heads * self.head_dim
         if self._fused_qk(qkv, rope):
             qkv5 = qkv.view(b, n, 3, self.num_heads, self.head_dim)

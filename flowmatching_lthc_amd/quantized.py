@@ -25,10 +25,6 @@ class QuantizedRows(NamedTuple):
     scale: Tensor
     dtype: torch.dtype
 
-    @property
-    def shape(self) -> torch.Size:
-        return self.values.shape
-
 
 class Int8Linear(nn.Module):
     """nn.Linear for inference on 8-bit rows: weight int8 [out, in rounded up to a multiple of 16], weight_scale and bias fp32.

@@ -694,7 +694,8 @@ int lthc_norm_quantize(const void* x, int x_dtype, int64_t x_ld, const void* res
  *   h[m,n] = (sum_k q[m,k] weight[n,k]) q_scales[m] w_scales[n] + bias[n],  y = h
  * or, gated, weight [2F, K]: y[m,f] = act(h[m,f]) h[m,F+f].  Sums are exact (K up to 131056),
  * the rest fp32, rounded once to y_dtype.  bias fp32 or NULL.  K and the row strides are
- * multiples of 16, q and weight 16-byte aligned; any M, N and F.  y [M, N] ([M, F]).
+ * multiples of 16, the latter up to 2^22, q and weight 16-byte aligned; N (F) up to 2^20, any
+ * M.  y [M, N] ([M, F]), aligned to its elements.
  */
 int lthc_int8_linear(const int8_t* q, int64_t q_ld, const float* q_scales, const int8_t* weight, int64_t w_ld, const float* w_scales,
                      const float* bias, void* y, int y_dtype, int64_t M, int64_t N, int64_t K, void* stream);

@@ -238,6 +238,38 @@ def test_int8_gated_linear(act, m, f, k):
     check_gated(q, s, w, v, None, act, torch.bfloat16)
 
 
+# Sizes that take each of the kernel's tiles: many tiles a block, last tiles that are not whole, stages that are not.
+TILED = [
+    (16300, 1792, 2048),  # 256 x 256, two tiles a block
+    (13307, 1000, 2064),  # 256 x 256, y's rows not whole lines
+    (13312, 1002, 1040),  # 256 x 256 for such rows alone
+    (15300, 896, 16),  # 256 x 128, one stage
+    (15360, 897, 128),  # 256 x 128, an odd width
+    (30000, 1100, 784),  # 256 x 128, several tiles a block
+    (16384, 768, 272),  # 128 x 128
+    (4100, 1030, 400),  # 128 x 128, ragged
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", TILED)
+def test_int8_linear_tiles(dtype, m, n, k):
+    q, s, w, v, b = int8_case(m, n, k)
+    y = check_linear(q, s, w, v, b, dtype)
+    for _ in range(3):
+        assert torch.equal(ops_int8.int8_linear(q, s, w, v, b, dtype), y)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n,k", TILED)
+def test_int8_gated_linear_tiles(act, m, n, k):
+    q, s, w, v, b = int8_case(m, 2 * (n // 2), k)
+    dtype = {"silu": torch.bfloat16, "gelu": torch.float32, "gelu_tanh": torch.float16}[act]
+    y = check_gated(q, s, w, v, b, act, dtype)
+    for _ in range(3):
+        assert torch.equal(ops_int8.int8_gated_linear(q, s, w, v, b, act, dtype), y)
+
+
 @pytest.mark.parametrize("m", [2, 50, 300])
 def test_products_of_rows_of_any_layout(m):
     q, s, w, v, b = int8_case(m, 96, 160)
@@ -246,8 +278,9 @@ def test_products_of_rows_of_any_layout(m):
     wide[:, 32:192] = q
     wide_w = torch.randint(-128, 128, (96, 208), device=DEV, dtype=torch.int8)
     wide_w[:, 16:176] = w
+    far = torch.zeros(m, (1 << 22) + 16, device=DEV, dtype=torch.int8)[:, 64:224].copy_(q)  # rows past the kernel's distance
     odd = torch.zeros(m * 160 + 3, device=DEV, dtype=torch.int8)[3:].view(m, 160).copy_(q)
-    for a in (wide[:, 32:192], odd, q.t().contiguous().t()):
+    for a in (wide[:, 32:192], odd, far, q.t().contiguous().t()):
         for c in (w, wide_w[:, 16:176], w.t().contiguous().t()):
             assert torch.equal(ops_int8.int8_linear(a, s, c, v, b, torch.bfloat16), want)
     three = ops_int8.int8_linear(q.view(2, m // 2, 160), s.view(2, m // 2), w, v, b.bfloat16().float(), torch.bfloat16)

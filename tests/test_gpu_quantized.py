@@ -231,6 +231,17 @@ def test_operators_in_a_compiled_function():
         assert a.dtype == b.dtype and torch.equal(a, b)
 
 
+@torch.no_grad()
+def test_branch_compiled():
+    b = quantize_branches(branch()).to(torch.bfloat16)
+    rope = M.VisionRotaryEmbeddingFast(32, 8).to(DEV)
+    z, t6 = randn(2, 64, 256), 0.3 * randn(2, 6 * 256, seed=3)
+    want = b(z, t6, rope)
+    got = torch.compile(b, fullgraph=True)(z, t6, rope)
+    # the same operators; what is between them is views and copies
+    assert torch.equal(got, want)
+
+
 def test_a_recorded_call_is_refused():
     b = quantize_branches(branch())
     rope = M.VisionRotaryEmbeddingFast(32, 8).to(DEV)
