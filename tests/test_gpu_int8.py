@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from flowmatching_lthc_amd import ops_int8
+from flowmatching_lthc_amd import _abi, ops_int8
 
 pytestmark = pytest.mark.gpu
 
@@ -158,6 +158,26 @@ def test_norm_quantize_takes_rows_for_all_samples_other_types_and_two_dimensions
     wide = randn(4, 50, 320, dtype=torch.bfloat16, seed=9)
     check_norm(wide[:, :, 5:305], w, wide[:, :, 20:], g.contiguous(), sh, sc.contiguous(), "sum")
     check_norm(x.transpose(0, 1), w, r.transpose(0, 1), None, None, None, "sum")
+
+
+@pytest.mark.parametrize("keep", ["sum", "update"])
+@pytest.mark.parametrize("c", [768, 1100, 9001])  # a row in registers of a wavefront, of a block, and longer ones
+def test_what_is_kept_may_take_the_place_of_an_operand(keep, c):
+    x, w, r, g, sh, sc = norm_case(2, 21, c, torch.bfloat16, True, True, True)
+    want = ops_int8.norm_quantize(x, w, 1e-6, r, g, sh, sc, keep)
+    lib, k = _abi.load(), ops_int8.padded(c)
+    for place in ("residual", "x"):
+        to = {"residual": r.clone(), "x": x.clone()}
+        kept, a, b = to[place], to["x"], to["residual"]
+        q, s = torch.zeros(42, k, device=DEV, dtype=torch.int8), torch.zeros(42, device=DEV)
+        rc = lib.lthc_norm_quantize(
+            a.data_ptr(), _abi.BF16, c, b.data_ptr(), c, g.data_ptr(), _abi.BF16, g.stride(0), w.data_ptr(), _abi.F32, sh.data_ptr(),
+            sc.data_ptr(), _abi.BF16, sh.stride(0), {"sum": 1, "update": 2}[keep], kept.data_ptr(), q.data_ptr(), k, s.data_ptr(), 2, 21, c,
+            1e-6, torch.cuda.current_stream().cuda_stream,
+        )  # fmt: skip
+        _abi.check(rc, "lthc_norm_quantize")
+        for got, w_ in zip((kept, q, s), want):
+            assert torch.equal(got.view(-1), w_.reshape(-1))
 
 
 def test_norm_quantize_of_zeros():

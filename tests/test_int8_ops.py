@@ -48,6 +48,15 @@ def test_row_entry_points_refuse_bad_arguments():
     assert norm(b=0, w=None) == _abi.OK
 
 
+def test_row_entry_points_refuse_sizes_whose_products_leave_64_bits():
+    lib, uns = _abi.load(), _abi.ERR_UNSUPPORTED
+    many = 1 << 60
+    refused(lib.lthc_quantize_rows(FAKE, 1, 16, FAKE, 16, FAKE, many, 16, None), uns, "rows")
+    refused(lib.lthc_dequantize_rows(FAKE, 16, FAKE, FAKE, 1, many, 16, None), uns, "rows")
+    for b, n in ((1 << 40, 1 << 30), (1 << 30, 1 << 30), (1 << 20, 1 << 40)):
+        refused(lib.lthc_norm_quantize(FAKE, 1, 16, None, 0, None, 0, 0, FAKE, 0, None, None, 0, 0, 0, None, FAKE, 16, FAKE, b, n, 16, 1e-6, None), uns, "")
+
+
 @pytest.mark.parametrize("gated", [False, True])
 def test_product_entry_points_refuse_bad_arguments(gated):
     lib = _abi.load()
