@@ -19,11 +19,16 @@ from . import ops_int8
 
 
 class QuantizedRows(NamedTuple):
-    """8-bit rows with their scales, and the dtype of the activations that they stand for."""
+    """8-bit rows with their scales, and the dtype of a layer's result on them."""
 
     values: Tensor
     scale: Tensor
     dtype: torch.dtype
+
+
+def _dtype(x: Tensor) -> torch.dtype:
+    """The dtype of a linear layer's result on x: autocast's in its region."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
 class Int8Linear(nn.Module):
@@ -63,8 +68,7 @@ class Int8Linear(nn.Module):
     def rows(self, x: Tensor | QuantizedRows) -> QuantizedRows:
         if isinstance(x, QuantizedRows):
             return x
-        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-        return QuantizedRows(*ops_int8.quantize_rows(x), dtype)
+        return QuantizedRows(*ops_int8.quantize_rows(x), _dtype(x))
 
     def forward(self, x: Tensor | QuantizedRows) -> Tensor:
         q, scale, dtype = self.rows(x)
@@ -81,7 +85,7 @@ def norm_rows(
 ) -> tuple[Tensor, QuantizedRows]:
     """(kept, modulate(norm(residual + gate * x), shift, scale) as 8-bit rows): ops_int8.norm_quantize of an RMSNorm."""
     kept, q, s = ops_int8.norm_quantize(x, norm.weight, norm.eps, residual, gate, shift, scale, keep)
-    return kept, QuantizedRows(q, s, x.dtype)
+    return kept, QuantizedRows(q, s, _dtype(x))
 
 
 def quantize_branches(model: nn.Module) -> nn.Module:

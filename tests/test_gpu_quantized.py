@@ -78,6 +78,19 @@ def branch(dim=256, heads=4, seed=1, cls=M.WorkspaceSharedAdaLNBranch):
     return b.to(DEV).eval()
 
 
+@torch.no_grad()
+def test_norms_rows_stand_for_autocasts_dtype():
+    b = branch()
+    z, row = randn(2, 64, 256, dtype=torch.float32), randn(2, 256, dtype=torch.float32, seed=1)
+    want = {None: torch.float32, torch.bfloat16: torch.bfloat16, torch.float16: torch.float16}
+    plain = copy.deepcopy(b)
+    b.attn.qkv = Int8Linear.from_linear(b.attn.qkv)
+    for cast, dtype in want.items():
+        with torch.autocast("cuda", cast or torch.bfloat16, enabled=cast is not None):
+            rows = b.attention_input(z, row, row)
+            assert isinstance(rows, QuantizedRows) and b.attn.qkv(rows).dtype == plain.attn.qkv(plain.attention_input(z, row, row)).dtype == dtype
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @torch.no_grad()
 def test_branch_runs_the_8_bit_operators(dtype):
