@@ -261,13 +261,22 @@ def test_int8_gated_linear(act, m, f, k):
 # Sizes that take each of the kernel's tiles: many tiles a block, last tiles that are not whole, stages that are not.
 TILED = [
     (16300, 1792, 2048),  # 256 x 256, two tiles a block
-    (13307, 1000, 2064),  # 256 x 256, y's rows not whole lines
-    (13312, 1002, 1040),  # 256 x 256 for such rows alone
-    (15300, 896, 16),  # 256 x 128, one stage
+    (14500, 1000, 2064),  # 256 x 256, y's rows not whole lines
+    (14592, 1002, 1040),  # 256 x 256 for such rows alone
+    (14500, 1001, 2096),  # 256 x 256, an odd width
+    (16300, 896, 16),  # 256 x 128, one stage
     (15360, 897, 128),  # 256 x 128, an odd width
-    (30000, 1100, 784),  # 256 x 128, several tiles a block
-    (16384, 768, 272),  # 128 x 128
-    (4100, 1030, 400),  # 128 x 128, ragged
+    (30000, 1200, 784),  # 256 x 128, several tiles a block
+    (13307, 1000, 2064),  # 128 x 128, and so are the following
+    (13312, 1002, 1040),
+    (15300, 896, 16),
+    (30000, 1100, 784),
+    (16384, 768, 272),
+    (4100, 1030, 400),
+    (2000, 1100, 784),  # 128 x 64
+    (1030, 1450, 2064),
+    (700, 2305, 128),
+    (1000, 1102, 784),  # 64 x 64
 ]
 
 
