@@ -87,6 +87,23 @@ def test_rows_of_any_layout():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [4, 30, 200, 300, 700, 1000, 1500, 2047, 3500, 4096, 8100, 16001, 16400])
+def test_rows_at_any_address_of_an_element(dtype, c):
+    wide = randn(11, c + 3, dtype=dtype) * 3
+    for first in (0, 1, 2, 3):
+        x = wide[:, first : first + c]
+        q, s = ops_int8.quantize_rows(x)
+        want, ws = ops_int8.quantize_rows(x.contiguous())
+        check_rows(q, s, x.double(), torch.zeros(11, 1, device=DEV, dtype=torch.float64))
+        assert torch.equal(q, want) and torch.equal(s, ws)
+        back = ops_int8.dequantize_rows(q, s, c, dtype)
+        assert torch.equal(back, ops_int8.dequantize_rows(q.clone(), s, q.shape[1], dtype)[:, :c])
+        w = 1 + 0.1 * randn(c, seed=3)
+        for keep in ("sum", "update"):
+            assert all(torch.equal(a, b) for a, b in zip(ops_int8.norm_quantize(x, w, 1e-6, x, w, keep=keep), ops_int8.norm_quantize(x.contiguous(), w, 1e-6, x.contiguous(), w, keep=keep)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,c,k", [(1, 1, 16), (13, 37, 48), (300, 768, 768), (7, 2730, 2736)])
 def test_dequantize_rows(dtype, m, c, k):
     q = torch.randint(-128, 128, (m, k), device=DEV, dtype=torch.int8, generator=torch.Generator(device=DEV).manual_seed(1))
