@@ -88,8 +88,8 @@ def int8_gated_linear_eager(
 @torch.library.custom_op("jit_thc::quantize_rows", mutates_args=())
 def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
     """(q, scale) of x [..., C], fp32, bf16 or fp16: scale = max(max |x| / 127, 2^-126) of each row, q = rint(x / scale) as
-    int8 [..., padded(C)], zeros past C; rows of 512 elements and more lie a multiple of 128 apart.  A value within 2^-21
-    (relative) of a tie goes to either side.  A row with a NaN or an infinity has the scale NaN and q 0."""
+    int8 [..., padded(C)], zeros past C; rows of 512 elements and more lie a multiple of 128 apart.  Both quotients are
+    fp32, ties go to the even integer.  A row with a NaN or an infinity has the scale NaN and q 0."""
     _refuse(x)
 
 

@@ -659,7 +659,7 @@ int lthc_grad_norm(const void* const* grads, int g_dtype, const int64_t* numels,
  *   s[m] = max(max_c |x[m,c]| / 127, 2^-126),  q[m,c] = rint(x[m,c] / s[m])
  * q: int8 [M, Cp], Cp = C rounded up to a multiple of 16, zeros past C, rows q_ld
  * elements apart (a multiple of 16; of 128 where the products should load whole lines);
- * scales: fp32 [M].  A value within 2^-21 (relative) of a tie goes to either side.  A row
+ * scales: fp32 [M].  Both quotients are fp32, rint's ties go to the even integer.  A row
  * with a NaN or an infinity: s = NaN, q = 0.
  * Back: out[m,c] = q[m,c] s[m] in out_dtype, [M, C].
  */
