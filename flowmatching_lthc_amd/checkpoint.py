@@ -55,7 +55,7 @@ def load_model_state(model: torch.nn.Module, ckpt: Mapping, key: str = "ema") ->
 
     ``key="model"`` loads the full state dict strictly.  ``key="ema"`` takes every entry the EMA holds (the
     EMA stores parameters only) and keeps the model's own values for the rest, such as buffers; the names
-    kept are returned.  Old key names are migrated first (names the model itself has are kept as they are).
+    kept are returned.  An 8-bit layer that takes a weight from the EMA takes its scales from it too.  Old key names are migrated first (names the model itself has are kept as they are).
     Raises ``ValueError`` for another key and ``KeyError`` when the checkpoint has no EMA weights.
     """
     own = set(model.state_dict())
@@ -69,9 +69,11 @@ def load_model_state(model: torch.nn.Module, ckpt: Mapping, key: str = "ema") ->
     ema = migrate_checkpoint_state(ckpt["ema"], own)
     state = model.state_dict()
     kept = []
-    for name in state:
+    for name in list(state):
         if name in ema:
             state[name] = ema[name]
+        elif name.endswith(".weight_scale") and name.removesuffix("_scale") in ema:  # Int8Linear's, found from that weight
+            del state[name]
         else:
             kept.append(name)
     model.load_state_dict(state)

@@ -31,11 +31,20 @@ def _dtype(x: Tensor) -> torch.dtype:
     return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
+@torch.no_grad()
+def _weight_rows(weight: Tensor) -> tuple[Tensor, Tensor]:
+    """(values, scales) of a linear layer's weight, the same on the CPU and on the GPU."""
+    w = weight.detach()
+    w = w if w.dtype in (torch.float32, torch.bfloat16, torch.float16) else w.float()
+    return ops_int8.quantize_rows(w) if w.is_cuda else ops_int8.quantize_rows_eager(w)
+
+
 class Int8Linear(nn.Module):
     """nn.Linear for inference on 8-bit rows: weight int8 [out, in rounded up to a multiple of 16], weight_scale and bias fp32.
 
     forward takes activations (quantised here) or QuantizedRows and returns the activations' dtype (autocast's in its
-    region).  weight_scale and bias stay fp32 when the module is converted to another dtype."""
+    region).  weight_scale and bias stay fp32 when the module is converted to another dtype.  A state dict holds the 8-bit
+    values with their scales; a linear layer's is taken too, and its weight quantised."""
 
     def __init__(self, weight: Tensor, weight_scale: Tensor, bias: Tensor | None, in_features: int) -> None:
         super().__init__()
@@ -46,11 +55,26 @@ class Int8Linear(nn.Module):
         self.register_buffer("bias", bias)
 
     @classmethod
-    @torch.no_grad()
     def from_linear(cls, layer: nn.Linear) -> Int8Linear:
-        w = layer.weight.detach()
-        q, scale = ops_int8.quantize_rows(w) if w.is_cuda else ops_int8.quantize_rows_eager(w)
-        return cls(q, scale, None if layer.bias is None else layer.bias.detach().float().clone(), layer.in_features)
+        return cls(*_weight_rows(layer.weight), None if layer.bias is None else layer.bias.detach().float().clone(), layer.in_features)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs) -> None:
+        """A linear layer's weight is quantised on the way; 8-bit values and their scales come together."""
+        names = [prefix + n for n in ("weight", "weight_scale")]
+        w, scale = (state_dict.get(n) for n in names)
+        if w is not None and w.is_floating_point():
+            if w.shape != (self.out_features, self.in_features):
+                error_msgs.append(f"{names[0]}: [{self.out_features}, {self.in_features}] expected for a linear layer's weight, got {list(w.shape)}")
+                return
+            on = w.device if self.weight.is_meta else self.weight.device
+            state_dict = {**state_dict, **dict(zip(names, _weight_rows(w.to(on))))}
+            bias = state_dict.get(prefix + "bias")
+            if bias is not None:
+                state_dict[prefix + "bias"] = bias.float()
+        elif (w is None) != (scale is None) or (w is not None and w.dtype != torch.int8):
+            error_msgs.append(f"{names[0]}: a linear layer's weight, or int8 values with {names[1]}, expected")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
@@ -91,8 +115,8 @@ def norm_rows(
 def quantize_branches(model: nn.Module) -> nn.Module:
     """Replaces the linear layers of every workspace branch of `model` by Int8Linear, in place, and returns the model.
 
-    For inference: load the weights first (the state dict holds 8-bit weights afterwards), call the model under
-    torch.no_grad().  A layer that is not a plain linear layer (hooks, a parametrization, another class) is refused."""
+    For inference: call the model under torch.no_grad().  The state dict holds 8-bit weights afterwards; one of the model as it
+    was is taken too (Int8Linear).  A layer that is not a plain linear layer (hooks, a parametrization, another class) is refused."""
     from .model import SwiGLUFFN, WorkspaceAttention, _plain_projection
 
     found = [(m, n) for m in model.modules() if isinstance(m, WorkspaceAttention) for n in ("qkv", "proj")]
