@@ -92,6 +92,9 @@ class Int8Linear(nn.Module):
     def rows(self, x: Tensor | QuantizedRows) -> QuantizedRows:
         if isinstance(x, QuantizedRows):
             return x
+        # 8-bit rows are padded to multiples of 16, and so other widths would pass the product's own check
+        if x.dim() == 0 or x.shape[-1] != self.in_features:
+            raise ValueError(f"Int8Linear of {self.in_features} channels: [..., {self.in_features}] expected, got {list(x.shape)}")
         return QuantizedRows(*ops_int8.quantize_rows(x), _dtype(x))
 
     def forward(self, x: Tensor | QuantizedRows) -> Tensor:

@@ -33,3 +33,14 @@ def test_a_layer_takes_a_linear_layers_state(dtype, assign):
         q = q.to(DEV)
         assert q.weight.dtype == torch.int8 and q.weight_scale.dtype == q.bias.dtype == torch.float32
         assert torch.equal(q(x), want(x))
+
+
+@pytest.mark.parametrize("k", [5, 768, 2730])
+@torch.no_grad()
+def test_a_layer_refuses_other_widths(k):
+    layer = Int8Linear.from_linear(linear(k, 6))
+    assert layer(torch.zeros(2, k, device=DEV)).shape == (2, 6) and layer.gated(torch.zeros(2, k, device=DEV), "silu").shape == (2, 3)
+    for wrong in (k - 1, k + 1, layer.weight.shape[1] + 16):
+        for call in (layer, lambda x: layer.gated(x, "silu")):
+            with pytest.raises(ValueError, match=f"of {k} channels"):
+                call(torch.zeros(2, wrong, device=DEV))

@@ -114,3 +114,13 @@ def test_a_state_without_the_layer_leaves_it_as_it_is():
     assert_same(numbers(mine), before)
     with pytest.raises(RuntimeError, match="Missing"):
         mine.load_state_dict({})
+
+
+@pytest.mark.parametrize("k,wrong", [(768, 767), (768, 753), (2730, 2731), (2730, 2736), (2730, 2721), (5, 16), (16, 32)])
+def test_a_layer_refuses_other_widths(k, wrong):
+    layer = Int8Linear.from_linear(linear(k, 6))
+    for x in (torch.zeros(3, wrong), torch.zeros(wrong), torch.tensor(1.0)):
+        with pytest.raises(ValueError, match=f"of {k} channels"):
+            layer(x)
+        with pytest.raises(ValueError, match=f"of {k} channels"):
+            layer.gated(x, "silu")
