@@ -85,14 +85,26 @@ class RMSNorm(nn.Module):
         return (xf * inv * self.weight).to(x.dtype)
 
 
-def norm_modulate(norm: RMSNorm, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+def _watched(m: nn.Module) -> bool:
+    """Whether something else than the call sees or replaces what module m is called with."""
+    return bool(m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__) or nn.modules.module._has_any_global_hook()
+
+
+def _plain_norm(norm: nn.Module) -> bool:
+    """Whether calling `norm` is RMSNorm.forward and nothing else: no other forward, no hooks."""
+    return not (overridden(norm, "forward", RMSNorm) or _watched(norm) or norm._backward_hooks or norm._backward_pre_hooks)
+
+
+def norm_modulate(norm: nn.Module, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """modulate(norm(x), shift, scale) for x [B, N, C] and per-sample [B, C] shift / scale.
 
     On the GPU, when shift and scale share x's dtype (bf16 autocast or fp32), one HIP pass with the eager
     sequence's roundings (jit_thc::norm_modulate); otherwise the eager sequence itself (other dtype mixes
-    follow torch's promotion rules, which the kernel does not implement).
+    follow torch's promotion rules, which the kernel does not implement; a norm with hooks or a forward of its
+    own is called).
     """
-    if x.is_cuda and x.dim() == 3 and shift.dtype == x.dtype and scale.dtype == x.dtype and x.shape[-1] % 4 == 0 and x.shape[-1] <= 2048:
+    fits = x.is_cuda and x.dim() == 3 and shift.dtype == x.dtype and scale.dtype == x.dtype and x.shape[-1] % 4 == 0 and x.shape[-1] <= 2048
+    if fits and _plain_norm(norm):
         return ops.norm_modulate(x, norm.weight, shift, scale, norm.eps)[0]
     return modulate(norm(x), shift, scale)
 
@@ -405,18 +417,14 @@ class SwiGLUFFN(nn.Module):
         return self.w3(self.ffn_dropout(act))
 
 
-def _watched(m: nn.Module) -> bool:
-    """Whether something else than the call sees or replaces what module m is called with."""
-    return bool(m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__) or nn.modules.module._has_any_global_hook()
-
-
 def _takes_rows(module: nn.Module, name: str, norm: nn.Module, x: torch.Tensor) -> bool:
     """Whether `norm` on x can hand `module` (attention or feed-forward), whose first layer is `name`, its output as 8-bit
-    rows: an Int8Linear there, modules of this package that nothing watches, a GPU tensor of the operators' dtypes."""
+    rows: an Int8Linear there, modules of this package that nothing watches, the norm among them, a GPU tensor of the
+    operators' dtypes."""
     layer = module._modules.get(name) if type(module) in (WorkspaceAttention, SwiGLUFFN) else None
     return (
         type(layer) is Int8Linear
-        and type(norm) is RMSNorm
+        and _plain_norm(norm)
         and not (_watched(layer) or _watched(module))
         and x.is_cuda
         and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
@@ -465,6 +473,9 @@ class WorkspaceSharedAdaLNBranch(nn.Module):
         self, z: torch.Tensor, a: torch.Tensor, gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor
     ) -> tuple[torch.Tensor, torch.Tensor | QuantizedRows]:
         """(gate * a, the second pre-norm of z + gate * a), the latter as 8-bit rows where w12 takes them."""
+        if not _plain_norm(self.norm2):
+            d_attn = gate.unsqueeze(1) * a
+            return d_attn, norm_modulate(self.norm2, z + d_attn, shift, scale)
         if _takes_rows(self.mlp, "w12", self.norm2, z):
             return norm_rows(self.norm2, a, shift, scale, z, gate, "update")
         return ops_branch.gate_add_norm_modulate(z, a, gate, self.norm2.weight, shift, scale, self.norm2.eps)
@@ -965,6 +976,7 @@ class SharedReadLocalTHCSharedAdaLNJiT(BatchedWeightCast, nn.Module):
                 and "lazy_workspace_update" not in blk.__dict__
                 and type(blk.branch) is WorkspaceSharedAdaLNBranch
                 and "forward" not in blk.branch.__dict__
+                and _plain_norm(blk.branch.norm1)
             ):
                 return False
         return True
