@@ -51,6 +51,14 @@ class CastLinear(nn.Linear):
         y = ops_branch.linear(x, self.weight, self.bias)
         return y if y is not None else super().forward(x)
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs) -> None:
+        """An 8-bit layer's values, which stand for a weight with their scales alone, are refused."""
+        w = state_dict.get(prefix + "weight")
+        if isinstance(w, torch.Tensor) and not w.is_floating_point():
+            error_msgs.append(f"{prefix}weight: a floating-point weight expected, got {w.dtype} (quantize_branches the model before it loads 8-bit weights)")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
 
 def _plain_projection(layer: nn.Module) -> bool:
     """Whether calling `layer` is CastLinear.forward on its weight and bias and nothing else: no other class (a

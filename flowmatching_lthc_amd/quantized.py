@@ -62,7 +62,7 @@ class Int8Linear(nn.Module):
         """A linear layer's weight is quantised on the way; 8-bit values and their scales come together."""
         names = [prefix + n for n in ("weight", "weight_scale")]
         w, scale = (state_dict.get(n) for n in names)
-        if w is not None and w.is_floating_point():
+        if isinstance(w, Tensor) and w.is_floating_point():
             if w.shape != (self.out_features, self.in_features):
                 error_msgs.append(f"{names[0]}: [{self.out_features}, {self.in_features}] expected for a linear layer's weight, got {list(w.shape)}")
                 return

@@ -124,3 +124,15 @@ def test_a_layer_refuses_other_widths(k, wrong):
             layer(x)
         with pytest.raises(ValueError, match=f"of {k} channels"):
             layer.gated(x, "silu")
+
+
+@pytest.mark.parametrize("strict", [True, False])
+def test_a_linear_layer_refuses_8_bit_values(models, strict):
+    plain, quantised, _ = models
+    model = copy.deepcopy(plain)
+    before = numbers(model)
+    with pytest.raises(RuntimeError, match="quantize_branches"):
+        model.load_state_dict(quantised.state_dict(), strict=strict)
+    with pytest.raises(RuntimeError, match="quantize_branches"):
+        load_model_state(model, {"ema": quantised.state_dict()}, "ema")
+    assert all(torch.equal(t, before[n]) for n, t in model.state_dict().items() if ".branch." in n)
