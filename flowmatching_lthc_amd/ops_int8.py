@@ -51,7 +51,8 @@ def whole_lines(q: Tensor) -> Tensor:
 def quantize_rows_eager(x: Tensor) -> tuple[Tensor, Tensor]:
     x = x.float()
     top = x.abs().amax(-1)
-    scale = torch.where(top.isfinite(), (top / 127).clamp(min=TINY), torch.nan)
+    # by a tensor: a GPU tensor's quotient by a number is a product with the number's reciprocal
+    scale = torch.where(top.isfinite(), (top / torch.full_like(top, 127)).clamp(min=TINY), torch.nan)
     q = torch.where(scale.isnan().unsqueeze(-1), 0, torch.round(x / scale.unsqueeze(-1)))
     return torch.nn.functional.pad(q, (0, padded(x.shape[-1]) - x.shape[-1])).to(torch.int8), scale
 

@@ -63,3 +63,12 @@ def test_norm_quantize_divides(dtype, c):
     want, scale = divided(shift)
     assert torch.equal(s.cpu(), scale.unsqueeze(1).expand(17, 3))
     assert torch.equal(q[..., :c].cpu(), want.unsqueeze(1).expand(17, 3, c))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [60, 768, 2730])
+def test_the_eager_rows_are_the_same_on_either_device(dtype, c):
+    x = rows_with_ties(200, c, dtype, seed=2)
+    q, s = ops_int8.quantize_rows_eager(x.to(DEV))
+    want, scale = ops_int8.quantize_rows_eager(x)
+    assert torch.equal(q.cpu(), want) and torch.equal(s.cpu(), scale)
