@@ -55,7 +55,8 @@ def load_model_state(model: torch.nn.Module, ckpt: Mapping, key: str = "ema") ->
 
     ``key="model"`` loads the full state dict strictly.  ``key="ema"`` takes every entry the EMA holds (the
     EMA stores parameters only) and keeps the model's own values for the rest, such as buffers; the names
-    kept are returned.  An 8-bit layer that takes a weight from the EMA takes its scales from it too.  Old key names are migrated first (names the model itself has are kept as they are).
+    kept are returned.  An 8-bit layer that takes a weight from the EMA takes its scales from it too.  Old key names
+    are migrated first (names the model itself has are kept as they are).
     Raises ``ValueError`` for another key and ``KeyError`` when the checkpoint has no EMA weights.
     """
     own = set(model.state_dict())

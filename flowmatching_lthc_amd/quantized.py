@@ -71,7 +71,7 @@ class Int8Linear(nn.Module):
             bias = state_dict.get(prefix + "bias")
             if bias is not None:
                 state_dict[prefix + "bias"] = bias.float()
-        elif (w is None) != (scale is None) or (w is not None and w.dtype != torch.int8):
+        elif (w is None) != (scale is None) or (w is not None and getattr(w, "dtype", None) != torch.int8):
             error_msgs.append(f"{names[0]}: a linear layer's weight, or int8 values with {names[1]}, expected")
             return
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
